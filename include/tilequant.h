@@ -466,6 +466,85 @@ int tq_decode_attention_noalloc(const void* q, int64_t q_stride_b, int64_t q_str
                                 int dtype, int batch, int q_heads, int kv_heads, int head_dim, int max_len,
                                 float scale, void* stream);
 
+/* ---- paged INT8 KV cache ---------------------------------------------------
+ * No reference counterpart (the reference decodes over one static 16-bit
+ * cache, src/runtime/graph_decode.py:96-479).  The cache of one layer is
+ * `pages` pages of `block` tokens (a power of two, 16..1024; pages * block <
+ * 2^31), each cut into units of 16 tokens:
+ *   k_codes int8 [pages][kv_heads][block / 16][16][head_dim]
+ *   v_codes int8 [pages][kv_heads][block / 16][head_dim][16]   (transposed)
+ *   k_scales, v_scales fp32 [pages][kv_heads][block / 16]
+ * contiguous, the codes 16-byte aligned, head_dim 64 or 128.  A value is
+ * code * scale of its unit and kv head.  Token `at` of page p has slot
+ * p * block + at. */
+typedef struct tq_kv8_cache {
+  int8_t* k_codes;
+  int8_t* v_codes;
+  float* k_scales;
+  float* v_scales;
+  int pages, kv_heads, head_dim, block;
+} tq_kv8_cache;
+
+/* One step of the block tables of `rows` requests, all on the device: row b of
+ * `table` [rows, width] (row stride table_stride) lists the pages of its
+ * lengths[b] tokens; free_list [free_capacity] is a stack of free pages of
+ * which free_count[0] are valid.  In row order:
+ *   - rows with finished[b] != 0 (NULL: none) push their pages, in table order,
+ *     and have length 0 and entries -1 from then on;
+ *   - row b asks for n = max(new_tokens[b], 0) tokens and the pages they need
+ *     beyond those it has.  It is granted them iff length + n <= width * block,
+ *     the pages that rows 0..b ask for are free (a row that needs no page does
+ *     not wait for this), and the tokens that rows 0..b ask for are at most
+ *     max_tokens.  A row whose length would pass the table's width asks for
+ *     nothing; other refused rows count as asking.  Granted rows pop pages from
+ *     the top of the stack; a refused row is left as it was.
+ * Written: lengths, table, free_list, free_count, granted [rows] (0 / 1),
+ * query_start [rows + 1] (places of each row's new tokens in the lists below),
+ * slots and positions [max_tokens]: the new tokens' slots and positions in their
+ * sequences, in row order; behind the last token slots are -1, positions 0. */
+int tq_block_tables_step(const int32_t* new_tokens, const uint8_t* finished, int32_t* table, int64_t table_stride,
+                         int32_t* lengths, int32_t* free_list, int free_capacity, int32_t* free_count,
+                         int32_t* slots, int32_t* positions, int32_t* query_start, uint8_t* granted, int rows,
+                         int width, int block, int max_tokens, void* stream);
+
+/* Quantizes k, v [tokens, kv_heads, head_dim] (16-bit, strides in elements per
+ * token / head, unit stride inside a head, 16-byte aligned, strides multiples
+ * of 8) into their slots; slots outside the cache are skipped.  The new tokens
+ * of one unit stand next to each other in the list, and a unit holds the tokens
+ * below the first offset written (a unit written from offset 0 starts afresh).
+ * Per unit and head, in fp32 with a = max |x| of its new tokens (NaN as 0,
+ * infinities as the type's largest value; a < 2^-100 as 0):
+ *   s = max(s_old, a / 127);  codes rint(x * (1 / s)), 0 when s is 0;
+ *   older codes c become rint(c * (s_old / s)) when s > s_old. */
+int tq_kv8_append(const tq_kv8_cache* cache, const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                  int64_t v_stride_t, int64_t v_stride_h, int dtype, const int32_t* slots, int tokens, void* stream);
+
+/* code * scale of the listed slots, rounded to dtype, into k_out, v_out
+ * [n, kv_heads, head_dim] (strides as above); slots outside the cache give
+ * zeros. */
+int tq_kv8_read(const tq_kv8_cache* cache, const int32_t* slots, int n, int dtype, void* k_out, int64_t k_stride_n,
+                int64_t k_stride_h, void* v_out, int64_t v_stride_n, int64_t v_stride_h, void* stream);
+
+/* Attention over the cache.  Sequence b has lengths[b] tokens (at most max_len
+ * and width * block count) in the pages of table row b, and its queries are q
+ * rows query_start[b] .. query_start[b + 1] - 1 (query_start NULL: row b, one
+ * each; then tokens == batch and max_query == 1): the last n of its tokens,
+ * already appended.  Query i of n sees keys 0 .. lengths[b] - n + i:
+ *   out = softmax(scale * q k^T) v,  kv head h / (q_heads / kv_heads)
+ * A query that sees no key gives zeros; keys whose table entry is not a page of
+ * the cache are left out; q rows of no sequence, and queries past max_query of
+ * their sequence, leave out as it was.  q, out: [tokens, q_heads, head_dim] with
+ * strides per token / head, 16-byte aligned, strides multiples of 8; at most 128
+ * query heads per kv head.  fp32 accumulation.  workspace =
+ * tq_kv8_attention_workspace_elems() floats, 8-byte aligned (0: none needed). */
+int64_t tq_kv8_attention_workspace_elems(int tokens, int batch, int q_heads, int kv_heads, int head_dim,
+                                         int max_query, int max_len);
+int tq_kv8_attention(const tq_kv8_cache* cache, const void* q, int64_t q_stride_t, int64_t q_stride_h, int dtype,
+                     const int32_t* table, int64_t table_stride, int width, const int32_t* lengths,
+                     const int32_t* query_start, int tokens, int batch, int q_heads, int max_query, int max_len,
+                     float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* workspace,
+                     int64_t workspace_elems, void* stream);
+
 /* ---- warming the next decode GEMM's weights into the right L2 ---------------
  * On MI355X each of the 8 XCDs has its own L2, and workgroups are dealt to
  * the XCDs round-robin by workgroup id.  The decode GEMM's schedule reads row

@@ -158,6 +158,23 @@ class PromptDesc(ctypes.Structure):
 _SIGNATURES["tq_prompt_forward"] = (_i, [ctypes.POINTER(PromptDesc)])
 
 
+class Kv8Cache(ctypes.Structure):
+    """Mirror of tq_kv8_cache (include/tilequant.h)."""
+
+    _fields_ = [("k_codes", _p), ("v_codes", _p), ("k_scales", _p), ("v_scales", _p),
+                ("pages", _i), ("kv_heads", _i), ("head_dim", _i), ("block", _i)]
+
+
+_SIGNATURES.update({
+    "tq_block_tables_step": (_i, [_p, _p, _p, _i64, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "tq_kv8_append": (_i, [ctypes.POINTER(Kv8Cache), _p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _p]),
+    "tq_kv8_read": (_i, [ctypes.POINTER(Kv8Cache), _p, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p]),
+    "tq_kv8_attention_workspace_elems": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
+    "tq_kv8_attention": (_i, [ctypes.POINTER(Kv8Cache), _p, _i64, _i64, _i, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _i,
+                              ctypes.c_float, _p, _i64, _i64, _p, _i64, _p]),
+})
+
+
 class L2Warm(ctypes.Structure):
     """Mirror of tq_l2_warm (include/tilequant.h): the next decode GEMM's
     packed tiles and row pointers, and the producer's extra workgroup count.
