@@ -676,6 +676,27 @@ int tq_greedy_step(const void* logits, int64_t logits_stride, int dtype, int bat
                    int64_t generated_stride, int generated_len, int64_t* position, int prompt_len,
                    int32_t* seq_used, void* stream);
 
+/* Draws one token per row of logits [rows, vocab] (bf16, fp16 or fp32, row
+ * stride logits_stride, any alignment of the element; vocab <= 500000) with
+ * the given number uniform[b] in [0, 1).  Tokens are taken in the order of
+ * descending logit, equal ones by ascending index, w_i = exp((z_i - z_max) / T):
+ *   top-k keeps the first k (k <= 0 or >= vocab: all), of mass W_k;
+ *   top-p keeps those before which the mass is < p * W_k (p >= 1: all);
+ *   min-p keeps those with w_i >= m; the first is always kept;
+ *   the answer is the first kept one whose inclusive mass is > uniform[b] * W,
+ *   W the mass of the kept (the last kept one if there is none).
+ * NaN logits count as -infinity, which is never drawn; where +infinity occurs
+ * only those tokens are drawn.  T <= 0 or NaN, or nothing to draw: torch.argmax's
+ * answer, as in tq_greedy_step.  Weights are multiples of 2^-40 of the largest
+ * and summed exactly, so the answer does not depend on the order of summation.
+ * Each setting comes per row (temperature, top_k, top_p, min_p [rows]) or, where
+ * that pointer is NULL, from its `_all` value.  No reference counterpart: the
+ * reference decodes greedily (src/runtime/graph_decode.py:347-385). */
+int tq_sample_tokens(const void* logits, int64_t logits_stride, int dtype, int rows, int vocab, const float* uniform,
+                     const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,
+                     const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* tokens,
+                     void* stream);
+
 /* ---- load-time packing -------------------------------------------------
  * w [m, k] (x_dtype, row stride w_stride_m) is read as if zero-padded to
  * multiples of 64.  tile_ids are flat ids r * n_tc + c.                  */
