@@ -691,11 +691,14 @@ int tq_greedy_step(const void* logits, int64_t logits_stride, int dtype, int bat
  * and summed exactly, so the answer does not depend on the order of summation.
  * Each setting comes per row (temperature, top_k, top_p, min_p [rows]) or, where
  * that pointer is NULL, from its `_all` value.  No reference counterpart: the
- * reference decodes greedily (src/runtime/graph_decode.py:347-385). */
+ * reference decodes greedily (src/runtime/graph_decode.py:347-385).
+ * rows <= 65535; workspace = tq_sample_workspace_elems() 64-bit elements (0: none
+ * needed; no initialisation). */
+int64_t tq_sample_workspace_elems(int rows, int vocab);
 int tq_sample_tokens(const void* logits, int64_t logits_stride, int dtype, int rows, int vocab, const float* uniform,
                      const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,
                      const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* tokens,
-                     void* stream);
+                     int64_t* workspace, int64_t workspace_elems, void* stream);
 
 /* ---- load-time packing -------------------------------------------------
  * w [m, k] (x_dtype, row stride w_stride_m) is read as if zero-padded to

@@ -28,7 +28,9 @@ def plain(z, u, t, k, p, m):
     if np.isneginf(z).all():
         return 0, 1.0
     order = np.argsort(-z, kind="stable")
-    w = np.exp((z[order] - z[order[0]]) / np.float64(t))
+    with np.errstate(invalid="ignore"):
+        w = np.exp((z[order] - z[order[0]]) / np.float64(t))
+    w = np.where(np.isneginf(z[order]), 0.0, w)         # also where t is infinite
     kept = k if 0 < k < n else n
     cum = np.cumsum(w)
     slack = 1.0
@@ -117,11 +119,12 @@ def test_ties_rank_by_index(dtype):
     check(z, u, p=0.9)
 
 
-def test_masked_infinite_and_nan_logits():
+@pytest.mark.parametrize("vocab", [500, 30000])
+def test_masked_infinite_and_nan_logits(vocab):
     inf, nan = float("inf"), float("nan")
-    z = torch.randn((9, 500), generator=torch.Generator().manual_seed(2))
+    z = torch.randn((9, vocab), generator=torch.Generator().manual_seed(2))
     z[0] = -inf                                       # nothing left: argmax's answer
-    z[1, :499] = -inf                                 # one left, the last
+    z[1, :-1] = -inf                                  # one left, the last
     z[2] = nan
     z[3, ::2] = nan
     z[4, 17] = z[4, 33] = z[4, 400] = inf             # equally likely, the others not at all
@@ -135,12 +138,14 @@ def test_masked_infinite_and_nan_logits():
         for dt in (torch.float32, torch.bfloat16):
             got = check(z.to(dt), u, exact=True, **s)
             if s.get("t", 1.0) > 0:
-                assert got[0] == 0 and got[1] == 499 and got[4] in (17, 33, 400)
+                assert got[0] == 0 and got[1] == vocab - 1 and got[4] in (17, 33, 400)
     assert check(z, u, t=0.0)[2] == 0 and check(z, u, t=0.0)[3] == 0
 
 
-def test_odd_settings():
-    z, u = logits_like(7, 3001, torch.float32, seed=3)
+@pytest.mark.parametrize("vocab", [3001, 40000])
+def test_odd_settings(vocab):
+    z, u = logits_like(7, vocab, torch.float32, seed=3)
+    z[:, 5::7] = -float("inf")
     for s in (dict(t=float("inf")), dict(t=1e-30), dict(t=float("nan")), dict(t=-1.0), dict(p=0.0), dict(p=-1.0), dict(p=2.0),
               dict(m=1.0), dict(m=2.0), dict(k=-5), dict(k=2 ** 31 - 1), dict(k=3001), dict(k=3000), dict(t=1e30),
               dict(k=0, p=1e-9), dict(m=1e-30), dict(m=1e-40)):

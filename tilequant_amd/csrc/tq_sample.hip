@@ -14,26 +14,35 @@
 // distribution are as small as a token's probability (1e-6 and less), so masses are exact integers: w is computed in
 // fp64 and rounded to a multiple of 2^-40 (tokens below 2^-41 of the likeliest count as 0), and sums are 64-bit.
 //
-// One workgroup of 1024 threads per row.  The row is read two or more times (the second time from the caches); the
-// choice of path is by the row's settings:
+// Two ways through a row, by its settings:
 //   list   k <= 512, or min-p alone: a bound that at least k logits reach comes from the threads' maxima; the logits
 //          above it (a few more than k) are sorted in LDS, and all rules are applied there.
-//   bins   otherwise: one pass adds every token's count and mass to 128 bins of 0.3 octaves of w, then only the tokens of
-//          the bins where a target falls are sorted.  Bins are 128 columns wide, and a lane adds to the column of its
-//          number: no bank conflicts, no two lanes of a wave at one address.  A bin with more tokens than the list holds
-//          is divided by key until it fits or holds one value, whose ties are counted in index order.
+//   bins   otherwise: one pass adds every token's count and mass to 126 bins of 1/3 octave of w, then only the tokens of
+//          the bins where a target falls are looked at: they are narrowed down by key and index until at most 256 are
+//          left to sort.  Bins have 32 or more columns, and a lane adds to the column of its number: no bank conflicts, no
+//          two lanes at one address.
+// Short rows, and rows enough to fill the chip, take one launch of one workgroup per row.  Else a row is cut in C chunks
+// and there are three: the threads' maxima of every chunk; the chunk's list or bins, now that the row's maximum is known;
+// and one workgroup per row that finishes.  Masses being integers, C does not change the answer.
 #include "tq_common.h"
+
+#include <float.h>
 
 namespace tq {
 
-constexpr int kSampThreads = 1024;
+constexpr int kSampThreads = 1024;     // of the workgroup that finishes a row
 constexpr int kSampWaves = kSampThreads / kWave;
 constexpr int kSampBins = 128;
 constexpr int kSampCols = 128;
+constexpr int kChunkThreads = 256;     // of a chunk's workgroup
+constexpr int kChunkCols = 32;
+constexpr int kChunkList = 2048;       // list entries that the chunks of a row may hand over
 constexpr int kSampList = 8192;        // entries of the sorted list: 8 bytes of key and index, 8 of prefix mass
 constexpr int kSampTopK = 512;         // largest k of the list path: half the threads' maxima
+constexpr int kSampSort = 256;         // entries sorted by rank
 constexpr int kSampBoundBins = 512;
 constexpr int kSampMaxVocab = 500000;  // a column's count has 12 bits: 1024 threads deal at most 4095 tokens to a column
+constexpr int kChunkMost = 120000;     // tokens of a chunk, for the same reason
 constexpr int kSampWhole = 2048;       // the bins down to the last one needed are sorted together up to this many tokens
 constexpr uint64_t kSampCount = 1ull << 52;    // one token in a column's word: count above bit 52, mass below
 
@@ -49,6 +58,15 @@ struct SampleArgs {
   int top_k0;
   int64_t* out;
   int rows, vocab;
+  // the split form's workspace, per row
+  int chunks;
+  float* maxima;        // [chunks * kChunkThreads]
+  uint64_t* bin_mass;   // [chunks][kSampBins]
+  uint64_t* list;       // [kChunkList]
+  uint64_t* above_mass; // [chunks]: mass and number of the tokens with w >= m
+  uint32_t* above;
+  uint32_t* bin_count;  // [chunks][kSampBins]
+  uint32_t* n_list;     // [1]
 };
 
 struct F32In {
@@ -98,60 +116,98 @@ __device__ inline double exp2_small(double x) {
   return __builtin_ldexp(r, (int)n);
 }
 
+// A row's settings.
+struct SampleSettings {
+  float T;
+  int k;         // 0: all
+  double p, m;
+  float u;
+  __device__ SampleSettings(const SampleArgs& a, int b) {
+    T = a.temperature ? a.temperature[b] : a.temperature0;
+    k = a.top_k ? a.top_k[b] : a.top_k0;
+    if (k <= 0 || k >= a.vocab) k = 0;
+    p = a.top_p ? a.top_p[b] : a.top_p0;
+    m = a.min_p ? a.min_p[b] : a.min_p0;
+    u = a.u[b];
+  }
+  __device__ bool greedy() const { return !(T > 0.0f); }
+  __device__ bool by_list() const { return (k > 0 && k <= kSampTopK) || (k == 0 && p >= 1.0 && m > 0.0); }
+};
+
 // The row as its settings see it.
 struct SampleRow {
-  float top;       // z_max
-  bool infinite;   // z_max is +infinity: z becomes 0 there and -infinity elsewhere (top is 0 then)
-  double c;        // log2(e) / T
-  __device__ inline float see(float z) const {   // NaN -> -infinity
-    if (infinite) return z == INFINITY ? 0.0f : -INFINITY;
-    return z == z ? z : -INFINITY;
+  float top;             // z_max
+  bool infinite;         // z_max is +infinity: z becomes 0 there and -infinity elsewhere (top is 0 then)
+  double c, top64;       // log2 w = (z - z_max) c, c = log2(e) / T; the difference first: z c alone may be huge
+  float half_top, step;  // 3 log2(w) = -(half_top - z / 2) step, which does not overflow
+  __device__ SampleRow(float z_max, float T) {   // the same in all lanes: kept in scalar registers
+    z_max = uniform(z_max);
+    infinite = z_max == INFINITY;
+    top = infinite ? 0.0f : z_max;
+    c = uniform(1.4426950408889634074 / (double)T);
+    top64 = uniform((double)top);
+    half_top = uniform(0.5f * top);
+    step = uniform((float)fmin(6.0 * c, 3.0e38));
   }
-  __device__ inline double x(float z) const { return z == -INFINITY ? -1e30 : ((double)z - (double)top) * c; }
-  __device__ inline double weight(float z) const {
-    const double v = x(z);
-    return v < -42.0 ? 0.0 : exp2_small(v);
+  __device__ static inline float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
+  __device__ static inline double uniform(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b), hi = __builtin_amdgcn_readfirstlane((int)(b >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
   }
+  __device__ inline float see(float z) const { return !infinite ? z : z == INFINITY ? 0.0f : -INFINITY; }
+  // The place among the bins: bin i holds place in [i, i + 1).  Ascends as z descends; from 126 on (w < 2^-42) a token
+  // counts as nothing, and for NaN and -infinity no comparison holds.
+  __device__ inline float place(float z) const { return fmaf(z, -0.5f, half_top) * step; }
+  __device__ static inline bool alive(float place) { return place < 126.0f; }
+  __device__ inline double log2_weight(float z) const { return ((double)z - top64) * c; }
+  __device__ inline double weight(float z) const { return alive(place(z)) ? exp2_small(log2_weight(z)) : 0.0; }
   // the weight in 2^-40: adding 2^12 leaves it in the low bits of the mantissa, rounded to nearest
   __device__ static inline uint64_t mass(double w) {
     return __builtin_bit_cast(uint64_t, w + 4096.0) & (kSampCount - 1);
   }
-  __device__ static inline int bin(double v) { return min((int)(v * -3.0), kSampBins - 1); }
 };
+
+// Bins and what lies before each.
+template <int N>
+struct Bins {
+  uint64_t mass[N], mass_before[N];
+  uint32_t count[N], before[N];
+};
+constexpr int kWorkBins = 64;          // of a turn that narrows a search down
 
 struct SampleShared {
   float red_f[kSampWaves];
   uint64_t red_u[kSampWaves];
   int red_i[kSampWaves];
   uint32_t bound[kSampBoundBins];
-  uint32_t bin_count[kSampBins];
-  uint64_t bin_mass[kSampBins];      // then: before each bin
-  uint32_t bin_before[kSampBins];
-  uint64_t mass_before[kSampBins];
-  int n_list, found, found_index;
-  uint32_t lo, hi;
-  uint64_t found_before, found_mass;
+  Bins<kSampBins> row;
+  Bins<kWorkBins> work;
+  int n_list, found;
+  unsigned long long first, last;
 };
 
+template <int NT = kSampThreads>
 __device__ inline float block_max_f(float v, float* red) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = red[threadIdx.x & (kSampWaves - 1)];
+  v = red[threadIdx.x & (NT / kWave - 1)];
 #pragma unroll
-  for (int o = kSampWaves / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  for (int o = NT / kWave / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   __syncthreads();
   return v;
 }
+template <int NT = kSampThreads>
 __device__ inline uint64_t block_sum(uint64_t v, uint64_t* red) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = red[threadIdx.x & (kSampWaves - 1)];
+  v = red[threadIdx.x & (NT / kWave - 1)];
 #pragma unroll
-  for (int o = kSampWaves / 2; o; o >>= 1) v += __shfl_xor(v, o);
+  for (int o = NT / kWave / 2; o; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
   return v;
 }
@@ -174,12 +230,11 @@ __device__ inline uint64_t block_before(uint64_t v, uint64_t* red) {
 
 // f(z, i) for the vectors vec0, vec0 + step, .. of the row: 16-byte aligned loads from the one that holds the row's first
 // element on; what they hold beside the row is given as -infinity with an index out of range.
-template <class IN, class F>
-__device__ inline void sweep(const typename IN::T* row, int vocab, int vec0, int vec1, int step, F f) {
+template <class IN, int kBatch, class F>
+__device__ __forceinline__ void sweep(const typename IN::T* row, int vocab, int vec0, int vec1, int step, F f) {
   constexpr int V = IN::kVec;
   const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(typename IN::T));
   const u32x4* base = reinterpret_cast<const u32x4*>(row - off);
-  constexpr int kBatch = 4;
   for (int j0 = vec0; j0 < vec1; j0 += step * kBatch) {
     u32x4 w[kBatch];
 #pragma unroll
@@ -206,10 +261,10 @@ __device__ inline int row_vectors(const typename IN::T* row, int vocab) {
 
 // torch.argmax: NaN first, then the largest, the lowest index among equals.
 template <class IN>
-__device__ inline int argmax_row(const typename IN::T* row, int vocab, SampleShared& sh) {
+__device__ __forceinline__ int argmax_row(const typename IN::T* row, int vocab, SampleShared& sh) {
   float best = -INFINITY;
   int at = 0x7fffffff;
-  sweep<IN>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
+  sweep<IN, 2>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
 #pragma unroll
     for (int e = 0; e < IN::kVec; ++e) {
       const int i = i0 + e;
@@ -246,26 +301,31 @@ __device__ inline int argmax_row(const typename IN::T* row, int vocab, SampleSha
 }
 
 // ---- the sorted list ------------------------------------------------------------
-// list[i] = (~key) << 32 | index: ascending order is the order of the tokens.  n entries at any place; afterwards sorted.
-__device__ inline void sort_list(uint64_t* list, uint64_t* spare, int n) {
-  const int t = threadIdx.x;
-  if (n <= 256) {   // by rank: four threads per entry, each against a quarter of the others
-    const int e = t >> 2, part = t & 3;
-    uint64_t mine = ~0ull;
-    int rank = 0;
-    if (e < n) {
-      mine = list[e];
-      for (int j = part; j < n; j += 4) rank += list[j] < mine;
-    }
-    rank += __shfl_xor(rank, 1);
-    rank += __shfl_xor(rank, 2);
-    if (e < n && part == 0) spare[rank] = mine;
-    __syncthreads();
-    if (t < n) list[t] = spare[t];
-    __syncthreads();
-    return;
+// A token's place in the order as one number: (~key) << 32 | index ascends with it.
+__device__ inline uint64_t entry_of(float z, int i) { return (uint64_t)~key_of(z) << 32 | (uint32_t)i; }
+__device__ inline float logit_of(uint64_t entry) { return of_key(~(uint32_t)(entry >> 32)); }
+
+// Sorts n entries; up to kSampSort by rank (four threads per entry, each against a quarter of the others, through spare),
+// more in a bitonic network.
+__device__ __forceinline__ void sort_small(uint64_t* list, uint64_t* spare, int n) {
+  const int t = threadIdx.x, e = t >> 2, part = t & 3;
+  uint64_t mine = ~0ull;
+  int rank = 0;
+  if (e < n) {
+    mine = list[e];
+    for (int j = part; j < n; j += 4) rank += list[j] < mine;
   }
-  int size = 512;
+  rank += __shfl_xor(rank, 1);
+  rank += __shfl_xor(rank, 2);
+  if (e < n && part == 0) spare[rank] = mine;
+  __syncthreads();
+  if (t < n) list[t] = spare[t];
+  __syncthreads();
+}
+__device__ __forceinline__ void sort_list(uint64_t* list, uint64_t* spare, int n) {
+  if (n <= kSampSort) return sort_small(list, spare, n);
+  const int t = threadIdx.x;
+  int size = 2 * kSampSort;
   while (size < n) size <<= 1;
   for (int i = n + t; i < size; i += kSampThreads) list[i] = ~0ull;
   __syncthreads();
@@ -284,14 +344,17 @@ __device__ inline void sort_list(uint64_t* list, uint64_t* spare, int n) {
 }
 
 // prefix[i] = mass of the entries 0 .. i
-__device__ inline void sum_list(const uint64_t* list, uint64_t* prefix, int n, const SampleRow& r, SampleShared& sh) {
+__device__ __forceinline__ void sum_list(const uint64_t* list, uint64_t* prefix, int n, const SampleRow& r,
+                                         SampleShared& sh) {
   const int per = (n + kSampThreads - 1) / kSampThreads, i0 = threadIdx.x * per, i1 = min(i0 + per, n);
   uint64_t sum = 0;
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) {
-    sum += SampleRow::mass(r.weight(of_key(~(uint32_t)(list[i] >> 32))));
+    sum += SampleRow::mass(r.weight(logit_of(list[i])));
     prefix[i] = sum;
   }
   const uint64_t before = block_before(sum, sh.red_u);
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) prefix[i] += before;
   __syncthreads();
 }
@@ -308,20 +371,21 @@ __device__ inline int first_past(const uint64_t* prefix, int n, uint64_t base, d
   return lo;
 }
 
-// Adds the row's tokens that `take(z, key)` accepts to the list.  The list holds kSampList entries; sh.n_list is their number
-// also where it is more.
+// Puts the row's tokens that `take(z, entry)` accepts in the list, which holds kSampList; sh.n_list is their number also
+// where it is more.
 template <class IN, class F>
-__device__ inline void collect(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* list, SampleShared& sh,
-                               F take) {
+__device__ __forceinline__ void collect(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* list,
+                                        SampleShared& sh, F take) {
   if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
-  sweep<IN>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
+  sweep<IN, 2>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
 #pragma unroll
     for (int e = 0; e < IN::kVec; ++e) {
       const float v = r.see(z[e]);
-      if (v != -INFINITY && take(v)) {
+      const uint64_t entry = entry_of(v, i0 + e);
+      if (take(v, entry)) {
         const int at = atomicAdd(&sh.n_list, 1);
-        if (at < kSampList) list[at] = (uint64_t)~key_of(v) << 32 | (uint32_t)(i0 + e);
+        if (at < kSampList) list[at] = entry;
       }
     }
   });
@@ -330,8 +394,8 @@ __device__ inline void collect(const typename IN::T* row, int vocab, const Sampl
 
 // Applies the rules to a sorted list that is the whole beginning of the order.  w_k: the mass top-p is a part of, or
 // ~0 for that of the list's first k.
-__device__ inline int draw_from_list(const uint64_t* list, const uint64_t* prefix, int n, int k, double p, double m, double u,
-                                     uint64_t w_k, const SampleRow& r) {
+__device__ __forceinline__ int draw_from_list(const uint64_t* list, const uint64_t* prefix, int n, int k, double p, double m,
+                                              double u, uint64_t w_k, const SampleRow& r) {
   int kept = k > 0 ? min(k, n) : n;
   if (p < 1.0) {
     const double all = (double)(w_k == ~0ull ? prefix[kept - 1] : w_k);
@@ -341,7 +405,7 @@ __device__ inline int draw_from_list(const uint64_t* list, const uint64_t* prefi
     int lo = 0, hi = kept;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (r.weight(of_key(~(uint32_t)(list[mid] >> 32))) >= m) lo = mid + 1;
+      if (r.weight(logit_of(list[mid])) >= m) lo = mid + 1;
       else hi = mid;
     }
     kept = lo;
@@ -352,33 +416,22 @@ __device__ inline int draw_from_list(const uint64_t* list, const uint64_t* prefi
 }
 
 // ---- bins -----------------------------------------------------------------------
-// Counts and masses of up to kSampBins bins over the tokens for which bin_of(z, x) >= 0; prefix sums in sh.
-template <class IN, class F>
-__device__ inline void fill_bins(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells, SampleShared& sh,
-                                 F bin_of) {
+// A token's word for its bin's cell.
+__device__ inline void add_to_cell(uint64_t* cell, double w) {
+  atomicAdd((unsigned long long*)cell, (unsigned long long)(SampleRow::mass(w) + kSampCount));
+}
+
+// Counts and masses of the bins, their columns summed up, by 8 threads each.
+template <int BINS, int COLS>
+__device__ __forceinline__ void sum_cells(const uint64_t* cells, Bins<BINS>& out) {
   const int t = threadIdx.x;
-  for (int i = t; i < kSampBins * kSampCols; i += kSampThreads) cells[i] = 0;
-  __syncthreads();
-  uint64_t* mine = cells + (t & (kSampCols - 1));
-  sweep<IN>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int) {
-#pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) {
-      const float v = r.see(z[e]);
-      const double x = r.x(v);
-      if (x >= -42.0) {
-        const double w = exp2_small(x);
-        const int b = bin_of(v, x, w);
-        if (b >= 0) atomicAdd((unsigned long long*)&mine[b * kSampCols], (unsigned long long)(SampleRow::mass(w) + kSampCount));
-      }
-    }
-  });
-  __syncthreads();
-  {
+  if (t < BINS * 8) {
     const int b = t >> 3, part = t & 7;
     uint64_t mass = 0;
     uint32_t count = 0;
-    for (int i = 0; i < kSampCols / 8; ++i) {
-      const uint64_t c = cells[b * kSampCols + part + 8 * i];
+#pragma unroll 1
+    for (int i = 0; i < COLS / 8; ++i) {
+      const uint64_t c = cells[b * COLS + part + 8 * i];
       mass += c & (kSampCount - 1);
       count += (uint32_t)(c >> 52);
     }
@@ -388,16 +441,26 @@ __device__ inline void fill_bins(const typename IN::T* row, int vocab, const Sam
       count += __shfl_xor(count, o);
     }
     if (part == 0) {
-      sh.bin_count[b] = count;
-      sh.bin_mass[b] = mass;
+      out.count[b] = count;
+      out.mass[b] = mass;
     }
   }
   __syncthreads();
-  if (t < kWave) {   // prefix sums: lane takes bins 2 t and 2 t + 1
-    const uint32_t c0 = sh.bin_count[2 * t], c1 = sh.bin_count[2 * t + 1];
-    const uint64_t m0 = sh.bin_mass[2 * t], m1 = sh.bin_mass[2 * t + 1];
-    uint32_t c = c0 + c1;
-    uint64_t m = m0 + m1;
+}
+template <int BINS>
+__device__ __forceinline__ void before_bins(Bins<BINS>& b) {
+  constexpr int kPer = BINS / kWave;
+  const int t = threadIdx.x;
+  if (t < kWave) {
+    uint32_t c = 0;
+    uint64_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      c += b.count[kPer * t + i];
+      m += b.mass[kPer * t + i];
+    }
+    const uint32_t c_own = c;
+    const uint64_t m_own = m;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
       const uint32_t cy = __shfl_up(c, o);
@@ -407,10 +470,15 @@ __device__ inline void fill_bins(const typename IN::T* row, int vocab, const Sam
         m += my;
       }
     }
-    sh.bin_before[2 * t] = c - c0 - c1;
-    sh.bin_before[2 * t + 1] = c - c1;
-    sh.mass_before[2 * t] = m - m0 - m1;
-    sh.mass_before[2 * t + 1] = m - m1;
+    c -= c_own;
+    m -= m_own;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      b.before[kPer * t + i] = c;
+      b.mass_before[kPer * t + i] = m;
+      c += b.count[kPer * t + i];
+      m += b.mass[kPer * t + i];
+    }
   }
   __syncthreads();
 }
@@ -420,6 +488,9 @@ struct Search {
   bool by_rank, or_equal;
   int64_t rank;
   double target;
+  __device__ inline bool past(int64_t count, uint64_t mass) const {   // of the tokens up to and with some token
+    return by_rank ? count > rank : or_equal ? (double)mass >= target : (double)mass > target;
+  }
 };
 struct Found {
   int64_t rank;      // of the token
@@ -427,209 +498,282 @@ struct Found {
   uint64_t through;  // mass of the tokens up to it, itself included
 };
 
-// The bin of a search among those of the last fill_bins (base: what lies before bin 0); the last that holds a token if none.
-__device__ inline int bin_of_search(const Search& s, const SampleShared& sh, int64_t base_count, uint64_t base_mass) {
-  const int lane = threadIdx.x & 63;   // bins 2 lane and 2 lane + 1
-  bool some[2], past[2];
+// The bin where a search stops (base: what lies before bin 0), or the last that holds a token; every wave finds it.
+template <int BINS>
+__device__ __forceinline__ int bin_of_search(const Search& s, const Bins<BINS>& bins, int64_t base_count,
+                                             uint64_t base_mass) {
+  constexpr int kPer = BINS / kWave;
+  const int lane = threadIdx.x & 63;   // bins kPer lane ..
+  int first = -1, last = -1;           // of this lane's: past, holding a token
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int b = 2 * lane + i;
-    some[i] = sh.bin_count[b] != 0;
-    const int64_t c = base_count + sh.bin_before[b] + sh.bin_count[b];
-    const double m = (double)(base_mass + sh.mass_before[b] + sh.bin_mass[b]);
-    past[i] = some[i] && (s.by_rank ? c > s.rank : s.or_equal ? m >= s.target : m > s.target);
+  for (int i = kPer - 1; i >= 0; --i) {
+    const int b = kPer * lane + i;
+    if (bins.count[b] == 0) continue;
+    if (last < 0) last = b;
+    if (s.past(base_count + bins.before[b] + bins.count[b], base_mass + bins.mass_before[b] + bins.mass[b])) first = b;
   }
-  const uint64_t first = __ballot(past[0] || past[1]), even = __ballot(past[0]);
-  if (first) {
-    const int l = __builtin_ctzll(first);
-    return 2 * l + ((even >> l) & 1 ? 0 : 1);
-  }
-  const uint64_t any = __ballot(some[0] || some[1]), odd = __ballot(some[1]);
-  if (!any) return 0;
-  const int l = 63 - __builtin_clzll(any);
-  return 2 * l + ((odd >> l) & 1 ? 1 : 0);
+  const uint64_t p = __ballot(first >= 0), h = __ballot(last >= 0);
+  if (p) return __builtin_amdgcn_readlane(first, __builtin_ctzll(p));
+  return h ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(h)) : 0;
 }
 
-// The search's token within the tokens `in(z, x)` accepts, `count` of them, after base_count tokens of base_mass.
-template <class IN, class F>
-__device__ inline Found search_in(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* list, uint64_t* prefix,
-                                  SampleShared& sh, const Search& s, int64_t base_count, uint64_t base_mass, uint32_t count,
-                                  F in) {
+// The bins of a whole row; above, above_mass: number and mass of the tokens with w >= m.
+template <class IN>
+__device__ __forceinline__ void fill_bins(const typename IN::T* row, int vocab, const SampleRow& r, double m, uint64_t* cells,
+                                          SampleShared& sh, uint64_t& above, uint64_t& above_mass) {
   const int t = threadIdx.x;
-  uint32_t lo = 0, hi = 0xffffffffu;   // keys
-  if (count > kSampList) {
-    if (t == 0) {
-      sh.lo = 0xffffffffu;
-      sh.hi = 0;
-    }
-    __syncthreads();
-    uint32_t a = 0xffffffffu, b = 0;
-    sweep<IN>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int) {
+  for (int i = t; i < kSampBins * kSampCols; i += kSampThreads) cells[i] = 0;
+  __syncthreads();
+  uint64_t* mine = cells + (t & (kSampCols - 1));
+  uint64_t n = 0, mass = 0;
+  sweep<IN, 1>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int) {
 #pragma unroll
-      for (int e = 0; e < IN::kVec; ++e) {
-        const float v = r.see(z[e]);
-        if (v != -INFINITY && in(v)) {
-          a = min(a, key_of(v));
-          b = max(b, key_of(v));
+    for (int e = 0; e < IN::kVec; ++e) {
+      const float v = r.see(z[e]), place = r.place(v);
+      if (SampleRow::alive(place)) {
+        const double w = exp2_small(r.log2_weight(v));
+        if (w >= m) {
+          n += 1;
+          mass += SampleRow::mass(w);
         }
+        add_to_cell(&mine[(int)place * kSampCols], w);
       }
-    });
-    atomicMin(&sh.lo, a);
-    atomicMax(&sh.hi, b);
-    __syncthreads();
-    lo = sh.lo;
-    hi = sh.hi;
-    __syncthreads();
-    while (count > kSampList && lo != hi) {   // the range shrinks 64-fold or more each time
-      int shift = 0;
-      while (((hi - lo) >> shift) >= kSampBins) ++shift;
-      fill_bins<IN>(row, vocab, r, list, sh, [&](float v, double, double) {
-        const uint32_t k = key_of(v);
-        return k >= lo && k <= hi && in(v) ? (int)((hi - k) >> shift) : -1;
-      });
-      const int b = bin_of_search(s, sh, base_count, base_mass);
-      base_count += sh.bin_before[b];
-      base_mass += sh.mass_before[b];
-      count = sh.bin_count[b];
-      hi -= (uint32_t)b << shift;
-      const uint32_t width = (1u << shift) - 1;
-      lo = hi - lo > width ? hi - width : lo;
-      __syncthreads();   // the next fill writes the bins
     }
-  }
-  if (count > kSampList) {   // one value: its ties in index order
-    const uint64_t each = SampleRow::mass(r.weight(of_key(lo)));
-    int64_t j;
-    if (s.by_rank) j = s.rank - base_count;
-    else {
-      int64_t a = 0, b = count - 1;
-      while (a < b) {
-        const int64_t mid = (a + b) >> 1;
-        const double m = (double)(base_mass + (uint64_t)(mid + 1) * each);
-        if (s.or_equal ? m >= s.target : m > s.target) b = mid;
-        else a = mid + 1;
-      }
-      j = a;
-    }
-    j = min(max(j, (int64_t)0), (int64_t)count - 1);
-    // each thread counts a stretch of the row; the one that holds the j-th tie names it
-    const int nvec = row_vectors<IN>(row, vocab), per = (nvec + kSampThreads - 1) / kSampThreads;
-    const int v0 = min(t * per, nvec), v1 = min(v0 + per, nvec);
-    uint32_t n = 0;
-    const auto tie = [&](float z) {
-      const float v = r.see(z);
-      return v != -INFINITY && key_of(v) == lo && in(v);
-    };
-    sweep<IN>(row, vocab, v0, v1, 1, [&](const auto& z, int) {
-#pragma unroll
-      for (int e = 0; e < IN::kVec; ++e) n += tie(z[e]);
-    });
-    int64_t before = (int64_t)block_before(n, sh.red_u);
-    if (before <= j && j < before + n)
-      sweep<IN>(row, vocab, v0, v1, 1, [&](const auto& z, int i0) {
-#pragma unroll
-        for (int e = 0; e < IN::kVec; ++e)
-          if (tie(z[e]) && before++ == j) sh.found_index = i0 + e;
-      });
-    __syncthreads();
-    const Found f{base_count + j, sh.found_index, base_mass + (uint64_t)(j + 1) * each};
-    __syncthreads();
-    return f;
-  }
-  collect<IN>(row, vocab, r, list, sh, [&](float v) {
-    const uint32_t k = key_of(v);
-    return k >= lo && k <= hi && in(v);
   });
-  const int n = min(sh.n_list, kSampList);
-  sort_list(list, prefix, n);
-  sum_list(list, prefix, n, r, sh);
-  int at = s.by_rank ? (int)min(s.rank - base_count, (int64_t)n - 1) : first_past(prefix, n, base_mass, s.target, s.or_equal);
+  __syncthreads();
+  sum_cells<kSampBins, kSampCols>(cells, sh.row);
+  before_bins(sh.row);
+  above = block_sum(n, sh.red_u);
+  above_mass = block_sum(mass, sh.red_u);
+}
+
+// Where a search stops in the row, its bins being known.  The tokens of the bin are narrowed down, 64 ranges of their
+// order (key, then index) at a time: over the row while they are more than the list holds, then in the list, until at
+// most kSampSort are left, which are sorted.  Each turn divides the range of 64-bit numbers by 32 or more.
+template <class IN>
+__device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells,
+                                            SampleShared& sh, const Search& s) {
+  const int t = threadIdx.x;
+  uint64_t* list = cells;
+  uint64_t* work = cells + kSampList;   // [kWorkBins][kSampCols], then the sorted entries' prefix masses
+  static_assert(kWorkBins * kSampCols == kSampList, "the turns' cells take the second half");
+  const int b = bin_of_search(s, sh.row, 0, 0);
+  const float from = (float)b, to = (float)(b + 1);
+  int64_t base_count = sh.row.before[b];
+  uint64_t base_mass = sh.row.mass_before[b];
+  int count = (int)sh.row.count[b], whole = 0;
+  uint64_t first = 0, last = ~0ull;
+  bool listed = false, ranged = false;
+  const auto in = [&](float v, uint64_t e) {
+    const float place = r.place(v);
+    return place >= from && place < to && e >= first && e <= last;
+  };
+  for (int turn = 0; turn < 20; ++turn) {   // 64 bits, 5 or more a turn, and one turn to list them
+    if (!listed && count <= kSampList) {
+      collect<IN>(row, vocab, r, list, sh, in);
+      whole = min(sh.n_list, kSampList);
+      listed = true;
+    }
+    if (count <= kSampSort) break;
+    if (!ranged) {   // the range that the tokens really take up
+      ranged = true;
+      unsigned long long lo = ~0ull, hi = 0;
+      if (listed) {
+        for (int i = t; i < whole; i += kSampThreads) {
+          const unsigned long long e = list[i];
+          lo = e < lo ? e : lo;
+          hi = e > hi ? e : hi;
+        }
+      } else {
+        sweep<IN, 1>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
+#pragma unroll
+          for (int e = 0; e < IN::kVec; ++e) {
+            const float v = r.see(z[e]);
+            const unsigned long long x = entry_of(v, i0 + e);
+            if (in(v, x)) {
+              lo = x < lo ? x : lo;
+              hi = x > hi ? x : hi;
+            }
+          }
+        });
+      }
+      if (t == 0) {
+        sh.first = ~0ull;
+        sh.last = 0;
+      }
+      __syncthreads();
+      atomicMin(&sh.first, lo);
+      atomicMax(&sh.last, hi);
+      __syncthreads();
+      first = sh.first;
+      last = sh.last;
+    }
+    const uint64_t range = last - first;   // at least kSampSort: the entries differ
+    const int shift = max(0, 58 - (int)__builtin_clzll(range | 1));
+    for (int i = t; i < kSampList; i += kSampThreads) work[i] = 0;
+    __syncthreads();
+    uint64_t* mine = work + (t & (kSampCols - 1));
+    if (listed) {
+#pragma unroll 1
+      for (int i = t; i < whole; i += kSampThreads) {
+        const uint64_t e = list[i];
+        if (e >= first && e <= last) add_to_cell(&mine[(int)((e - first) >> shift) * kSampCols], r.weight(logit_of(e)));
+      }
+    } else {
+      sweep<IN, 1>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
+#pragma unroll
+        for (int e = 0; e < IN::kVec; ++e) {
+          const float v = r.see(z[e]);
+          const uint64_t x = entry_of(v, i0 + e);
+          if (in(v, x)) add_to_cell(&mine[(int)((x - first) >> shift) * kSampCols], r.weight(v));
+        }
+      });
+    }
+    __syncthreads();
+    sum_cells<kWorkBins, kSampCols>(work, sh.work);
+    before_bins(sh.work);
+    const int w = bin_of_search(s, sh.work, base_count, base_mass);
+    base_count += sh.work.before[w];
+    base_mass += sh.work.mass_before[w];
+    count = (int)sh.work.count[w];
+    first += (uint64_t)w << shift;
+    const uint64_t end = first + ((1ull << shift) - 1);
+    last = end < last ? end : last;
+    const uint64_t end_of_key = first | 0xffffffffull;   // the rest of one key's indexes is empty
+    if (last <= end_of_key) {
+      const uint64_t most = (first & ~0xffffffffull) | (uint64_t)(uint32_t)vocab;
+      last = most < last ? most : last;
+    }
+    __syncthreads();   // the next turn writes the bins
+  }
+  // the entries in the range go to the work half
+  __syncthreads();   // every thread has read the list's length
+  if (t == 0) sh.n_list = 0;
+  __syncthreads();
+  for (int i = t; i < whole; i += kSampThreads) {
+    const uint64_t e = list[i];
+    if (e >= first && e <= last) {
+      const int at = atomicAdd(&sh.n_list, 1);
+      if (at < kSampSort) work[at] = e;
+    }
+  }
+  __syncthreads();
+  const int n = max(1, min(sh.n_list, kSampSort));
+  sort_small(work, list, n);
+  sum_list(work, list, n, r, sh);
+  int at = s.by_rank ? (int)(s.rank - base_count) : first_past(list, n, base_mass, s.target, s.or_equal);
   at = max(min(at, n - 1), 0);
-  const Found f{base_count + at, (int)(uint32_t)list[at], base_mass + prefix[at]};
-  __syncthreads();   // the list is written again
+  const Found f{base_count + at, (int)(uint32_t)work[at], base_mass + list[at]};
+  __syncthreads();   // both halves are written again
   return f;
 }
 
+// The answer of a row whose bins are in sh.row.
 template <class IN>
-__device__ inline int draw_from_bins(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells,
-                                     SampleShared& sh, int k, double p, double m, double u) {
-  uint64_t* list = cells;                 // the list takes the cells' place after they are summed up
-  uint64_t* prefix = cells + kSampList;
-  uint64_t above = 0, above_mass = 0;     // tokens with w >= m, of this thread
-  fill_bins<IN>(row, vocab, r, cells, sh, [&](float, double x, double w) {
-    if (w >= m) {
-      above += 1;
-      above_mass += SampleRow::mass(w);
-    }
-    return SampleRow::bin(x);
-  });
-  const int64_t total = (int64_t)sh.bin_before[kSampBins - 1] + sh.bin_count[kSampBins - 1];
-  const uint64_t total_mass = sh.mass_before[kSampBins - 1] + sh.bin_mass[kSampBins - 1];
+__device__ __forceinline__ int draw_from_bins(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells,
+                                              SampleShared& sh, const SampleSettings& set, uint64_t above,
+                                              uint64_t above_mass) {
+  const int64_t total = (int64_t)sh.row.before[kSampBins - 1] + sh.row.count[kSampBins - 1];
+  const uint64_t total_mass = sh.row.mass_before[kSampBins - 1] + sh.row.mass[kSampBins - 1];
   int64_t kept = total;
-  uint64_t kept_mass = total_mass;
-  const auto in_bin = [&](int b) { return [&r, b](float v) { const double x = r.x(v); return x >= -42.0 && SampleRow::bin(x) == b; }; };
-  const auto run = [&](const Search& s) {
-    const int b = bin_of_search(s, sh, 0, 0);
-    return search_in<IN>(row, vocab, r, list, prefix, sh, s, sh.bin_before[b], sh.mass_before[b], sh.bin_count[b], in_bin(b));
-  };
-  // the bins of the row, kept over searches that fill them again
-  __shared__ uint32_t count0[kSampBins], before0[kSampBins];
-  __shared__ uint64_t mass0[kSampBins], mbefore0[kSampBins];
-  if (threadIdx.x < kSampBins) {
-    count0[threadIdx.x] = sh.bin_count[threadIdx.x];
-    before0[threadIdx.x] = sh.bin_before[threadIdx.x];
-    mass0[threadIdx.x] = sh.bin_mass[threadIdx.x];
-    mbefore0[threadIdx.x] = sh.mass_before[threadIdx.x];
-  }
-  const auto restore = [&] {
-    __syncthreads();
-    if (threadIdx.x < kSampBins) {
-      sh.bin_count[threadIdx.x] = count0[threadIdx.x];
-      sh.bin_before[threadIdx.x] = before0[threadIdx.x];
-      sh.bin_mass[threadIdx.x] = mass0[threadIdx.x];
-      sh.mass_before[threadIdx.x] = mbefore0[threadIdx.x];
+  uint64_t kept_mass = total_mass, w_k = total_mass;
+  int answer = 0;
+#pragma unroll 1
+  for (int stage = 0; stage < 4; ++stage) {   // what top-k keeps, what top-p keeps, the number, the last that is kept
+    Search s{true, false, 0, 0.0};
+    if (stage == 0) {
+      if (!(set.k > 0 && set.k < total)) continue;
+      s.rank = set.k - 1;
+    } else if (stage == 1) {
+      if (!(set.p < 1.0)) continue;
+      s = Search{false, true, 0, set.p * (double)w_k};
+      const int b = bin_of_search(s, sh.row, 0, 0);
+      if ((int64_t)sh.row.before[b] + sh.row.count[b] <= kSampWhole) {   // all that can be kept, at once
+        const float to = (float)(b + 1);
+        collect<IN>(row, vocab, r, cells, sh, [&](float v, uint64_t) { return r.place(v) < to; });
+        const int n = max(1, min(sh.n_list, kSampList));
+        sort_list(cells, cells + kSampList, n);
+        sum_list(cells, cells + kSampList, n, r, sh);
+        const int k = set.k > 0 ? (int)(kept < n ? kept : n) : 0;
+        return draw_from_list(cells, cells + kSampList, n, k, set.p, set.m, set.u, w_k, r);
+      }
+    } else if (stage == 2) {
+      if (set.m > 0.0 && (int64_t)above < kept) {
+        kept = above > 0 ? (int64_t)above : 1;
+        kept_mass = above_mass;
+      }
+      // where nothing is likely enough the first token alone is kept
+      if (!(set.m > 0.0 && above == 0)) s = Search{false, false, 0, (double)set.u * (double)kept_mass};
+    } else {
+      s.rank = kept - 1;   // a number of 1 or more
     }
-    __syncthreads();
-  };
-  uint64_t w_k = total_mass;
-  if (k > 0 && k < total) {
-    const Found f = run(Search{true, false, k - 1, 0.0});
-    kept = k;
-    w_k = kept_mass = f.through;
-    restore();
-  }
-  if (p < 1.0) {
-    const Search s{false, true, 0, p * (double)w_k};
-    const int b = bin_of_search(s, sh, 0, 0);
-    const int64_t n = (int64_t)sh.bin_before[b] + sh.bin_count[b];
-    if (n <= kSampWhole) {   // all that can be kept, at once
-      const auto upto = [&r, b](float v) { const double x = r.x(v); return x >= -42.0 && SampleRow::bin(x) <= b; };
-      collect<IN>(row, vocab, r, list, sh, upto);
-      const int got = min(sh.n_list, kSampList);
-      sort_list(list, prefix, got);
-      sum_list(list, prefix, got, r, sh);
-      return draw_from_list(list, prefix, got, k > 0 ? (int)min(kept, (int64_t)got) : 0, p, m, u, w_k, r);
+    const Found f = search_row<IN>(row, vocab, r, cells, sh, s);
+    if (stage == 0) {
+      kept = set.k;
+      w_k = kept_mass = f.through;
+    } else if (stage == 1) {
+      if (f.rank + 1 < kept) {
+        kept = f.rank + 1;
+        kept_mass = f.through;
+      }
+    } else {
+      answer = f.index;
+      if (f.rank < kept) break;
     }
-    const Found f = run(s);
-    if (f.rank + 1 < kept) {
-      kept = f.rank + 1;
-      kept_mass = f.through;
-    }
-    restore();
   }
-  if (m > 0.0) {
-    const uint64_t n = block_sum(above, sh.red_u), s = block_sum(above_mass, sh.red_u);
-    if ((int64_t)n < kept && n > 0) {
-      kept = (int64_t)n;
-      kept_mass = s;
-    }
-    // nothing is that likely (m > 1): the first token alone
-    if (n == 0) return run(Search{true, false, 0, 0.0}).index;
+  return answer;
+}
+
+// The list path's bound: logits from here on make the list.  each(f) calls f on all of this thread's maxima.
+template <int NT, class F>
+__device__ inline float list_bound(const SampleSettings& set, const SampleRow& r, SampleShared& sh, F each) {
+  if (set.k == 0) {   // min-p alone: w >= m, a little below it for the rounding of the bound itself
+    const double z = (double)r.top + (set.m < 1.0 ? ((double)__builtin_amdgcn_logf((float)set.m) - 1e-4) / r.c : 0.0);
+    return fmaxf(fminf((float)(z - fabs(z) * 1e-6), r.top), -FLT_MAX);
   }
-  const Found f = run(Search{false, false, 0, u * (double)kept_mass});
-  if (f.rank < kept) return f.index;
-  restore();
-  return run(Search{true, false, kept - 1, 0.0}).index;   // u of 1 or more: the last that is kept
+  // the k-th largest of the threads' maxima, to a bin of (top - the smallest of them) / kSampBoundBins
+  float neg = -INFINITY;
+  each([&](float z) { neg = fmaxf(neg, z == -INFINITY ? -INFINITY : -z); });
+  const float low = -block_max_f<NT>(neg, sh.red_f);
+  const float half = 0.5f * r.top - 0.5f * low;   // does not overflow
+  const float s = half > 0.0f ? fminf((float)kSampBoundBins / half, 3.0e38f) : 0.0f;
+  const auto bin_of = [&](float z) { return min((int)((0.5f * r.top - 0.5f * z) * s), kSampBoundBins - 1); };
+  for (int i = threadIdx.x; i < kSampBoundBins; i += NT) sh.bound[i] = 0;
+  __syncthreads();
+  each([&](float z) {
+    if (z != -INFINITY) atomicAdd(&sh.bound[bin_of(z)], 1u);
+  });
+  __syncthreads();
+  const int t = threadIdx.x;
+  const uint32_t k = (uint32_t)set.k;
+  if (t < kWave) {
+    constexpr int kPer = kSampBoundBins / kWave;
+    uint32_t c[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += c[i] = sh.bound[t * kPer + i];
+    uint32_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t y = __shfl_up(inc, o);
+      if (t >= o) inc += y;
+    }
+    uint32_t before = inc - sum;
+    if (t == kWave - 1 && inc < k) sh.found = kSampBoundBins;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (before < k && before + c[i] >= k) sh.found = t * kPer + i;
+      before += c[i];
+    }
+  }
+  __syncthreads();
+  // the smallest of the maxima in the bins down to that one: at least k logits are as large
+  const int last = sh.found;
+  float mine = -INFINITY;
+  each([&](float z) {
+    if (z != -INFINITY && bin_of(z) <= last) mine = fmaxf(mine, -z);
+  });
+  const float bound = -block_max_f<NT>(mine, sh.red_f);
+  return last == kSampBoundBins ? -FLT_MAX : bound;   // fewer than k threads have one to show: all logits
 }
 
 template <class IN>
@@ -639,114 +783,268 @@ sample_kernel(SampleArgs a) {
   __shared__ SampleShared sh;
   const int t = threadIdx.x, b = blockIdx.x;
   const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
-  const float T = a.temperature ? a.temperature[b] : a.temperature0;
-  int k = a.top_k ? a.top_k[b] : a.top_k0;
-  const double p = a.top_p ? a.top_p[b] : a.top_p0;
-  const double m = a.min_p ? a.min_p[b] : a.min_p0;
-  const double u = a.u[b];
-  const auto answer = [&](int i) {
-    if (t == 0) a.out[b] = i;
-  };
-  if (!(T > 0.0f)) return answer(argmax_row<IN>(row, a.vocab, sh));
+  const SampleSettings set(a, b);
+  float mine = -INFINITY, top = -INFINITY;
+  if (!set.greedy()) {
+    sweep<IN, 4>(row, a.vocab, t, row_vectors<IN>(row, a.vocab), kSampThreads, [&](const auto& z, int) {
+#pragma unroll
+      for (int e = 0; e < IN::kVec; ++e) mine = fmaxf(mine, z[e]);   // passes over NaN
+    });
+    top = block_max_f(mine, sh.red_f);
+  }
+  int token = -1;
+  if (top == -INFINITY) {
+    token = argmax_row<IN>(row, a.vocab, sh);
+  } else {
+    const SampleRow r(top, set.T);
+    mine = r.see(mine);
+    if (set.by_list()) {
+      const float bound = list_bound<kSampThreads>(set, r, sh, [&](auto f) { f(mine); });
+      collect<IN>(row, a.vocab, r, cells, sh, [&](float v, uint64_t) { return v >= bound; });
+      const int n = sh.n_list;
+      if (n <= kSampList) {
+        sort_list(cells, cells + kSampList, n);
+        sum_list(cells, cells + kSampList, n, r, sh);
+        token = draw_from_list(cells, cells + kSampList, n, set.k, set.p, set.m, set.u, ~0ull, r);
+      }
+      __syncthreads();
+    }
+    if (token < 0) {
+      uint64_t above, above_mass;
+      fill_bins<IN>(row, a.vocab, r, set.m, cells, sh, above, above_mass);
+      token = draw_from_bins<IN>(row, a.vocab, r, cells, sh, set, above, above_mass);
+    }
+  }
+  if (t == 0) a.out[b] = token;
+}
 
+// ---- the split form ----------------------------------------------------------------
+__device__ inline void chunk_range(int nvec, int chunks, int chunk, int& v0, int& v1) {
+  const int per = (nvec + chunks - 1) / chunks;
+  v0 = min(chunk * per, nvec);
+  v1 = min(v0 + per, nvec);
+}
+
+template <class IN>
+__global__ void __launch_bounds__(kChunkThreads)
+sample_max_kernel(SampleArgs a) {
+  const int b = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
+  const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
+  int v0, v1;
+  chunk_range(row_vectors<IN>(row, a.vocab), a.chunks, c, v0, v1);
   float mine = -INFINITY;
-  sweep<IN>(row, a.vocab, t, row_vectors<IN>(row, a.vocab), kSampThreads, [&](const auto& z, int) {
+  sweep<IN, 4>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int) {
 #pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) mine = fmaxf(mine, z[e]);   // passes over NaN
+    for (int e = 0; e < IN::kVec; ++e) mine = fmaxf(mine, z[e]);
   });
-  SampleRow r;
-  r.top = block_max_f(mine, sh.red_f);
-  if (r.top == -INFINITY) return answer(argmax_row<IN>(row, a.vocab, sh));
-  r.infinite = r.top == INFINITY;
-  if (r.infinite) {
-    r.top = 0.0f;
-    mine = mine == INFINITY ? 0.0f : -INFINITY;
-  }
-  r.c = 1.4426950408889634074 / (double)T;
-  if (k <= 0 || k >= a.vocab) k = 0;
+  a.maxima[((int64_t)b * a.chunks + c) * kChunkThreads + t] = mine;
+  if (c == 0 && t == 0) a.n_list[b] = 0;
+}
 
-  uint64_t* list = cells;
-  uint64_t* prefix = cells + kSampList;
-  float bound = INFINITY;   // the list path's: logits from here on
-  if (k > 0 && k <= kSampTopK) {
-    // the k-th largest of the threads' maxima, to a bin of (top - the smallest of them) / kSampBoundBins
-    const float low = -block_max_f(mine == -INFINITY ? -INFINITY : -mine, sh.red_f);
-    const float s = r.top > low ? (float)kSampBoundBins / (r.top - low) : 0.0f;
-    const int bin = mine == -INFINITY ? kSampBoundBins : min((int)((r.top - mine) * s), kSampBoundBins - 1);
-    for (int i = t; i < kSampBoundBins; i += kSampThreads) sh.bound[i] = 0;
-    __syncthreads();
-    if (bin < kSampBoundBins) atomicAdd(&sh.bound[bin], 1u);
-    __syncthreads();
-    if (t < kWave) {
-      uint32_t c[kSampBoundBins / kWave], sum = 0;
+template <class IN>
+__global__ void __launch_bounds__(kChunkThreads)
+sample_chunk_kernel(SampleArgs a) {
+  __shared__ uint64_t cells[kSampBins * kChunkCols];
+  __shared__ SampleShared sh;
+  const int b = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
+  const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
+  const SampleSettings set(a, b);
+  if (set.greedy()) return;
+  const float* maxima = a.maxima + (int64_t)b * a.chunks * kChunkThreads;
+  float mine = -INFINITY;
+  for (int i = t; i < a.chunks * kChunkThreads; i += kChunkThreads) mine = fmaxf(mine, maxima[i]);
+  const float top = block_max_f<kChunkThreads>(mine, sh.red_f);
+  if (top == -INFINITY) return;
+  const SampleRow r(top, set.T);
+  int v0, v1;
+  chunk_range(row_vectors<IN>(row, a.vocab), a.chunks, c, v0, v1);
+  if (set.by_list()) {
+    const float bound = list_bound<kChunkThreads>(set, r, sh, [&](auto f) {
+      for (int i = t; i < a.chunks * kChunkThreads; i += kChunkThreads) f(r.see(maxima[i]));
+    });
+    uint64_t* list = a.list + (int64_t)b * kChunkList;
+    sweep<IN, 2>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int i0) {
 #pragma unroll
-      for (int i = 0; i < kSampBoundBins / kWave; ++i) sum += c[i] = sh.bound[t * (kSampBoundBins / kWave) + i];
-      uint32_t inc = sum;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) {
-        const uint32_t y = __shfl_up(inc, o);
-        if (t >= o) inc += y;
+      for (int e = 0; e < IN::kVec; ++e) {
+        const float v = r.see(z[e]);
+        if (v >= bound) {
+          const uint32_t at = atomicAdd(&a.n_list[b], 1u);
+          if (at < (uint32_t)kChunkList) list[at] = entry_of(v, i0 + e);
+        }
       }
-      uint32_t before = inc - sum;
-      if (t == kWave - 1) sh.found = inc < (uint32_t)k ? kSampBoundBins : sh.found;
-      __builtin_amdgcn_wave_barrier();
+    });
+    return;
+  }
+  for (int i = t; i < kSampBins * kChunkCols; i += kChunkThreads) cells[i] = 0;
+  __syncthreads();
+  uint64_t* own = cells + (t & (kChunkCols - 1));
+  uint64_t above = 0, above_mass = 0;
+  sweep<IN, 2>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int) {
 #pragma unroll
-      for (int i = 0; i < kSampBoundBins / kWave; ++i) {
-        if (before < (uint32_t)k && before + c[i] >= (uint32_t)k) sh.found = t * (kSampBoundBins / kWave) + i;
-        before += c[i];
+    for (int e = 0; e < IN::kVec; ++e) {
+      const float v = r.see(z[e]), place = r.place(v);
+      if (SampleRow::alive(place)) {
+        const double w = exp2_small(r.log2_weight(v));
+        if (w >= set.m) {
+          above += 1;
+          above_mass += SampleRow::mass(w);
+        }
+        add_to_cell(&own[(int)place * kChunkCols], w);
       }
     }
-    __syncthreads();
-    // the smallest of the maxima in the bins down to that one: at least k logits are as large
-    const int last = sh.found;
-    bound = -block_max_f(bin <= last && bin < kSampBoundBins ? -mine : -INFINITY, sh.red_f);
-    if (last == kSampBoundBins) bound = -INFINITY;   // fewer than k threads have one to show: all logits
-  } else if (k == 0 && p >= 1.0 && m > 0.0) {
-    // min-p alone: w >= m, a little below it for the rounding of the bound itself
-    const double z = (double)r.top + (m < 1.0 ? ((double)__builtin_amdgcn_logf((float)m) - 1e-4) / r.c : 0.0);
-    bound = fminf((float)(z - fabs(z) * 1e-6), r.top);
-  }
-  if (bound <= r.top) {
-    collect<IN>(row, a.vocab, r, list, sh, [&](float v) { return v >= bound; });
-    const int n = sh.n_list;
-    if (n <= kSampList && n > 0) {
-      sort_list(list, prefix, n);
-      sum_list(list, prefix, n, r, sh);
-      return answer(draw_from_list(list, prefix, n, k, p, m, u, ~0ull, r));
+  });
+  above = block_sum<kChunkThreads>(above, sh.red_u);   // and the barrier after the cells' additions
+  above_mass = block_sum<kChunkThreads>(above_mass, sh.red_u);
+  const int64_t at = (int64_t)b * a.chunks + c;
+  {
+    const int bin = t >> 1, part = t & 1;
+    uint64_t mass = 0;
+    uint32_t count = 0;
+    for (int i = 0; i < kChunkCols / 2; ++i) {
+      const uint64_t w = cells[bin * kChunkCols + 2 * i + part];
+      mass += w & (kSampCount - 1);
+      count += (uint32_t)(w >> 52);
     }
-    __syncthreads();
+    mass += __shfl_xor(mass, 1);
+    count += __shfl_xor(count, 1);
+    if (part == 0) {
+      a.bin_mass[at * kSampBins + bin] = mass;
+      a.bin_count[at * kSampBins + bin] = count;
+    }
   }
-  answer(draw_from_bins<IN>(row, a.vocab, r, cells, sh, k, p, m, u));
+  if (t == 0) {
+    a.above[at] = (uint32_t)above;
+    a.above_mass[at] = above_mass;
+  }
+}
+
+template <class IN>
+__global__ void __launch_bounds__(kSampThreads)
+sample_finish_kernel(SampleArgs a) {
+  extern __shared__ __align__(16) uint64_t cells[];
+  __shared__ SampleShared sh;
+  const int t = threadIdx.x, b = blockIdx.x;
+  const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
+  const SampleSettings set(a, b);
+  const float* maxima = a.maxima + (int64_t)b * a.chunks * kChunkThreads;
+  float top = -INFINITY;
+  if (!set.greedy()) {
+    for (int i = t; i < a.chunks * kChunkThreads; i += kSampThreads) top = fmaxf(top, maxima[i]);
+    top = block_max_f(top, sh.red_f);
+  }
+  int token;
+  if (top == -INFINITY) {
+    token = argmax_row<IN>(row, a.vocab, sh);
+  } else {
+    const SampleRow r(top, set.T);
+    const uint32_t listed = set.by_list() ? a.n_list[b] : ~0u;
+    if (listed <= (uint32_t)kChunkList) {
+      const int n = (int)listed;
+      for (int i = t; i < n; i += kSampThreads) cells[i] = a.list[(int64_t)b * kChunkList + i];
+      __syncthreads();
+      sort_list(cells, cells + kSampList, n);
+      sum_list(cells, cells + kSampList, n, r, sh);
+      token = draw_from_list(cells, cells + kSampList, n, set.k, set.p, set.m, set.u, ~0ull, r);
+    } else {
+      uint64_t above = 0, above_mass = 0;
+      if (set.by_list()) {   // more than the chunks could hand over
+        fill_bins<IN>(row, a.vocab, r, set.m, cells, sh, above, above_mass);
+      } else {
+        if (t < kSampBins) {
+          uint64_t mass = 0;
+          uint32_t count = 0;
+          for (int c = 0; c < a.chunks; ++c) {
+            mass += a.bin_mass[((int64_t)b * a.chunks + c) * kSampBins + t];
+            count += a.bin_count[((int64_t)b * a.chunks + c) * kSampBins + t];
+          }
+          sh.row.mass[t] = mass;
+          sh.row.count[t] = count;
+        }
+        for (int c = 0; c < a.chunks; ++c) {
+          above += a.above[(int64_t)b * a.chunks + c];
+          above_mass += a.above_mass[(int64_t)b * a.chunks + c];
+        }
+        __syncthreads();
+        before_bins(sh.row);
+      }
+      token = draw_from_bins<IN>(row, a.vocab, r, cells, sh, set, above, above_mass);
+    }
+  }
+  if (t == 0) a.out[b] = token;
+}
+
+// Chunks of a row, 0: one workgroup takes it whole.
+static int sample_chunks(int rows, int vocab) {
+  if (vocab < 16384) return 0;
+  int c = 1024 / rows;
+  c = c < 1 ? 1 : c > 32 ? 32 : c;
+  const int most = vocab / 2048, least = (vocab + kChunkMost - 1) / kChunkMost;
+  c = c > most ? most : c;
+  return c < least ? least : c;
+}
+
+// 8-byte words of the split form's workspace.
+static int64_t sample_words(int rows, int chunks) {
+  return (int64_t)rows * (chunks * (kChunkThreads / 2 + kSampBins + kSampBins / 2 + 2) + kChunkList + 1);
+}
+
+template <class IN>
+static int sample_launch(SampleArgs a, uint64_t* ws, hipStream_t s) {
+  constexpr size_t lds = (size_t)kSampBins * kSampCols * sizeof(uint64_t);
+  static_assert((size_t)kSampList * 16 == lds, "list and prefix take the bins' place");
+  if (a.chunks == 0) {
+    TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_kernel<IN>>(lds)));
+    hipLaunchKernelGGL(sample_kernel<IN>, dim3(a.rows), dim3(kSampThreads), lds, s, a);
+    return (int)hipGetLastError();
+  }
+  const int64_t n = (int64_t)a.rows * a.chunks;
+  a.bin_mass = ws;
+  a.list = a.bin_mass + n * kSampBins;
+  a.above_mass = a.list + (int64_t)a.rows * kChunkList;
+  a.maxima = reinterpret_cast<float*>(a.above_mass + n);
+  a.bin_count = reinterpret_cast<uint32_t*>(a.maxima + n * kChunkThreads);
+  a.above = a.bin_count + n * kSampBins;
+  a.n_list = a.above + n;
+  TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_finish_kernel<IN>>(lds)));
+  hipLaunchKernelGGL(sample_max_kernel<IN>, dim3(a.chunks, a.rows), dim3(kChunkThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_chunk_kernel<IN>, dim3(a.chunks, a.rows), dim3(kChunkThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_finish_kernel<IN>, dim3(a.rows), dim3(kSampThreads), lds, s, a);
+  return (int)hipGetLastError();
 }
 
 }  // namespace tq
 
 using namespace tq;
 
+extern "C" int64_t tq_sample_workspace_elems(int rows, int vocab) {
+  if (rows <= 0 || vocab <= 0 || vocab > kSampMaxVocab) return 0;
+  const int c = sample_chunks(rows, vocab);
+  return c ? sample_words(rows, c) : 0;
+}
+
 extern "C" int tq_sample_tokens(const void* logits, int64_t logits_stride, int dtype, int rows, int vocab,
                                 const float* uniform, const float* temperature, float temperature_all,
                                 const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
-                                const float* min_p, float min_p_all, int64_t* tokens, void* stream) {
+                                const float* min_p, float min_p_all, int64_t* tokens, int64_t* workspace,
+                                int64_t workspace_elems, void* stream) {
   if (dtype != TQ_DTYPE_BF16 && dtype != TQ_DTYPE_FP16 && dtype != TQ_DTYPE_FP32) return TQ_ERR_DTYPE;
-  if (rows < 0 || vocab <= 0 || vocab > kSampMaxVocab || (rows > 1 && logits_stride < vocab)) return TQ_ERR_ARG;
+  if (rows < 0 || rows > 65535 || vocab <= 0 || vocab > kSampMaxVocab || (rows > 1 && logits_stride < vocab))
+    return TQ_ERR_ARG;
   if (rows == 0) return TQ_OK;
   if (!logits || !uniform || !tokens) return TQ_ERR_ARG;
   const size_t size = dtype == TQ_DTYPE_FP32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size) return TQ_ERR_ALIGN;
-  const SampleArgs a{logits, logits_stride, uniform, temperature, top_k, top_p, min_p, temperature_all, top_p_all,
-                     min_p_all, top_k_all, tokens, rows, vocab};
-  constexpr size_t lds = (size_t)kSampBins * kSampCols * sizeof(uint64_t);
-  static_assert((size_t)kSampList * 16 == lds, "list and prefix take the bins' place");
+  SampleArgs a{};
+  a.x = logits; a.ld = logits_stride; a.u = uniform;
+  a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+  a.temperature0 = temperature_all; a.top_k0 = top_k_all; a.top_p0 = top_p_all; a.min_p0 = min_p_all;
+  a.out = tokens; a.rows = rows; a.vocab = vocab;
+  a.chunks = sample_chunks(rows, vocab);
+  if (a.chunks && (!workspace || workspace_elems < sample_words(rows, a.chunks))) return TQ_ERR_WORKSPACE;
+  uint64_t* ws = reinterpret_cast<uint64_t*>(workspace);
+  if (reinterpret_cast<uintptr_t>(ws) & 7u) return TQ_ERR_ALIGN;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == TQ_DTYPE_BF16) {
-    TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_kernel<H16In<Bf16>>>(lds)));
-    hipLaunchKernelGGL(sample_kernel<H16In<Bf16>>, dim3(rows), dim3(kSampThreads), lds, s, a);
-  } else if (dtype == TQ_DTYPE_FP16) {
-    TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_kernel<H16In<Fp16>>>(lds)));
-    hipLaunchKernelGGL(sample_kernel<H16In<Fp16>>, dim3(rows), dim3(kSampThreads), lds, s, a);
-  } else {
-    TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_kernel<F32In>>(lds)));
-    hipLaunchKernelGGL(sample_kernel<F32In>, dim3(rows), dim3(kSampThreads), lds, s, a);
-  }
-  return (int)hipGetLastError();
+  if (dtype == TQ_DTYPE_BF16) return sample_launch<H16In<Bf16>>(a, ws, s);
+  if (dtype == TQ_DTYPE_FP16) return sample_launch<H16In<Fp16>>(a, ws, s);
+  return sample_launch<F32In>(a, ws, s);
 }

@@ -1,7 +1,7 @@
 """Drawing tokens from logits (HIP, gfx950): temperature, top-k, top-p and min-p from given random numbers.
 
 ``sample_tokens`` stands beside the decoder's greedy step (``tq_greedy_step``; the reference decodes greedily only,
-src/runtime/graph_decode.py:347-385): one launch for any batch, every row with settings of its own, no host
+src/runtime/graph_decode.py:347-385): one call for any batch, every row with settings of its own, no host
 synchronisation, so it can be captured behind a model's logits.  The rules are in ``include/tilequant.h``
 (``tq_sample_tokens``), the kernel in ``csrc/tq_sample.hip``.
 """
@@ -59,9 +59,12 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
         out = torch.empty((rows,), dtype=torch.int64, device=logits.device)
     elif out.dtype != torch.int64 or out.shape != (rows,) or not out.is_contiguous() or out.device != logits.device:
         raise ValueError("out must be a contiguous int64 vector with one entry per row on the logits' device")
+    # scratch of this call alone: calls on other streams, and graphs, have their own
+    elems = int(nat.lib().tq_sample_workspace_elems(rows, vocab))
+    workspace = torch.empty((elems,), dtype=torch.int64, device=logits.device) if elems else None
     with torch.cuda.device(logits.device):
         rc = nat.lib().tq_sample_tokens(
             logits.data_ptr(), logits.stride(0), code, rows, vocab, uniform.data_ptr(), t, float(t_all), k, int(k_all), p,
-            float(p_all), m, float(m_all), out.data_ptr(), nat.stream_handle(logits.device))
+            float(p_all), m, float(m_all), out.data_ptr(), nat.ptr(workspace), elems, nat.stream_handle(logits.device))
     nat.check(rc, "tq_sample_tokens")
     return out
