@@ -687,7 +687,7 @@ int tq_greedy_step(const void* logits, int64_t logits_stride, int dtype, int bat
  *   W the mass of the kept (the last kept one if there is none).
  * NaN logits count as -infinity, which is never drawn; where +infinity occurs
  * only those tokens are drawn.  T <= 0 or NaN, or nothing to draw: torch.argmax's
- * answer, as in tq_greedy_step.  Weights are multiples of 2^-40 of the largest
+ * answer, as in tq_greedy_step.  Weights are multiples of 2^-39 of the largest
  * and summed exactly, so the answer does not depend on the order of summation.
  * Each setting comes per row (temperature, top_k, top_p, min_p [rows]) or, where
  * that pointer is NULL, from its `_all` value.  No reference counterpart: the

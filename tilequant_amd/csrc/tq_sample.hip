@@ -12,39 +12,41 @@
 //
 // Which token a number u falls on has to be the same whatever the order of summation, and the steps of the cumulative
 // distribution are as small as a token's probability (1e-6 and less), so masses are exact integers: w is computed in
-// fp64 and rounded to a multiple of 2^-40 (tokens below 2^-41 of the likeliest count as 0), and sums are 64-bit.
+// fp64 and rounded to a multiple of 2^-39 (tokens below 2^-40 of the likeliest count as 0), and sums are 64-bit.
 //
 // Two ways through a row, by its settings:
 //   list   k <= 512, or min-p alone: a bound that at least k logits reach comes from the threads' maxima; the logits
 //          above it (a few more than k) are sorted in LDS, and all rules are applied there.
-//   bins   otherwise: one pass adds every token's count and mass to 126 bins of 1/3 octave of w, then only the tokens of
+//   bins   otherwise: one pass adds every token's count and mass to 252 bins of 1/6 octave of w, then only the tokens of
 //          the bins where a target falls are looked at: they are narrowed down by key and index until at most 256 are
-//          left to sort.  Bins have 32 or more columns, and a lane adds to the column of its number: no bank conflicts, no
+//          left to sort.  Bins have 16 or more columns, and a lane adds to the column of its number: no bank conflicts, no
 //          two lanes at one address.
-// Short rows, and rows enough to fill the chip, take one launch of one workgroup per row.  Else a row is cut in C chunks
-// and there are three: the threads' maxima of every chunk; the chunk's list or bins, now that the row's maximum is known;
-// and one workgroup per row that finishes.  Masses being integers, C does not change the answer.
+// Short rows take one launch of one workgroup per row.  Others are cut in C chunks, and there are four:
+// maxima of every chunk; the chunk's list or bins, now that the row's maximum is known; the tokens of the bins that the
+// row's searches can end in, which the bins' sums tell, gathered; and one workgroup per row that finishes from the list
+// in LDS.  Masses being integers, C does not change the answer.
 #include "tq_common.h"
 
 #include <float.h>
 
 namespace tq {
 
-constexpr int kSampThreads = 1024;     // of the workgroup that finishes a row
+constexpr int kSampThreads = 512;      // of the workgroup that finishes a row
 constexpr int kSampWaves = kSampThreads / kWave;
-constexpr int kSampBins = 128;
-constexpr int kSampCols = 128;
+constexpr int kSampBins = 256;
+constexpr int kSampCols = 64;
 constexpr int kChunkThreads = 256;     // of a chunk's workgroup
-constexpr int kChunkCols = 32;
-constexpr int kChunkList = 2048;       // list entries that the chunks of a row may hand over
+constexpr int kChunkCols = 16;
+constexpr int kChunkList = 2048;       // list entries that one chunk may hand over
+constexpr int kMaxima = 2048;          // maxima of a row, at most
 constexpr int kSampList = 8192;        // entries of the sorted list: 8 bytes of key and index, 8 of prefix mass
 constexpr int kSampTopK = 512;         // largest k of the list path: half the threads' maxima
-constexpr int kSampSort = 256;         // entries sorted by rank
+constexpr int kSampSort = kSampThreads / 4;   // entries sorted by rank
 constexpr int kSampBoundBins = 512;
-constexpr int kSampMaxVocab = 500000;  // a column's count has 12 bits: 1024 threads deal at most 4095 tokens to a column
+constexpr int kSampMaxVocab = 500000;  // a column's count has 13 bits: at most 8191 tokens of a row per column
 constexpr int kChunkMost = 120000;     // tokens of a chunk, for the same reason
 constexpr int kSampWhole = 2048;       // the bins down to the last one needed are sorted together up to this many tokens
-constexpr uint64_t kSampCount = 1ull << 52;    // one token in a column's word: count above bit 52, mass below
+constexpr uint64_t kSampCount = 1ull << 51;    // one token in a column's word: count from bit 51 on, mass below
 
 struct SampleArgs {
   const void* x;
@@ -60,18 +62,30 @@ struct SampleArgs {
   int rows, vocab;
   // the split form's workspace, per row
   int chunks;
-  float* maxima;        // [chunks * kChunkThreads]
+  int per;              // maxima per chunk: of groups of kChunkThreads / per threads
+  int list_cap;
+  float* maxima;        // [chunks * per]; of a greedy row [chunks]: its best logits
+  int32_t* best;        // [chunks]: and where they are
   uint64_t* bin_mass;   // [chunks][kSampBins]
-  uint64_t* list;       // [kChunkList]
+  uint64_t* list;       // [list_cap]
   uint64_t* above_mass; // [chunks]: mass and number of the tokens with w >= m
   uint32_t* above;
   uint32_t* bin_count;  // [chunks][kSampBins]
   uint32_t* n_list;     // [1]
+  uint64_t* row_mass;   // [kSampBins + 2]: the row's bins, above_mass and above
+  uint32_t* row_count;  // [kSampBins]
 };
 
 struct F32In {
   using T = float;
   static constexpr int kVec = 4;
+  __device__ static inline float shift(u32x4& w) {   // the first element, the others one place down
+    const float f = __uint_as_float(w[0]);
+    w[0] = w[1];
+    w[1] = w[2];
+    w[2] = w[3];
+    return f;
+  }
   __device__ static inline void unpack(u32x4 w, float (&f)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
@@ -81,6 +95,14 @@ template <class XT>
 struct H16In {
   using T = uint16_t;
   static constexpr int kVec = 8;
+  __device__ static inline float shift(u32x4& w) {
+    const float f = XT::to_f32((uint16_t)(w[0] & 0xffffu));
+    w[0] = (w[0] >> 16) | (w[1] << 16);
+    w[1] = (w[1] >> 16) | (w[2] << 16);
+    w[2] = (w[2] >> 16) | (w[3] << 16);
+    w[3] >>= 16;
+    return f;
+  }
   __device__ static inline void unpack(u32x4 w, float (&f)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -122,13 +144,19 @@ struct SampleSettings {
   int k;         // 0: all
   double p, m;
   float u;
-  __device__ SampleSettings(const SampleArgs& a, int b) {
-    T = a.temperature ? a.temperature[b] : a.temperature0;
-    k = a.top_k ? a.top_k[b] : a.top_k0;
+  // Every load is made, from the numbers u where a setting has no vector, so that all go out together: a branch each
+  // would be a round trip to memory each.
+  __device__ __forceinline__ SampleSettings(const SampleArgs& a, int b) {
+    const float* any = a.u;
+    const float tv = (a.temperature ? a.temperature : any)[b], pv = (a.top_p ? a.top_p : any)[b];
+    const float mv = (a.min_p ? a.min_p : any)[b];
+    const int kv = (a.top_k ? a.top_k : reinterpret_cast<const int32_t*>(any))[b];
+    u = any[b];
+    T = a.temperature ? tv : a.temperature0;
+    k = a.top_k ? kv : a.top_k0;
     if (k <= 0 || k >= a.vocab) k = 0;
-    p = a.top_p ? a.top_p[b] : a.top_p0;
-    m = a.min_p ? a.min_p[b] : a.min_p0;
-    u = a.u[b];
+    p = a.top_p ? pv : a.top_p0;
+    m = a.min_p ? mv : a.min_p0;
   }
   __device__ bool greedy() const { return !(T > 0.0f); }
   __device__ bool by_list() const { return (k > 0 && k <= kSampTopK) || (k == 0 && p >= 1.0 && m > 0.0); }
@@ -139,7 +167,7 @@ struct SampleRow {
   float top;             // z_max
   bool infinite;         // z_max is +infinity: z becomes 0 there and -infinity elsewhere (top is 0 then)
   double c, top64;       // log2 w = (z - z_max) c, c = log2(e) / T; the difference first: z c alone may be huge
-  float half_top, step;  // 3 log2(w) = -(half_top - z / 2) step, which does not overflow
+  float half_top, step;  // 6 log2(w) = -(half_top - z / 2) step, which does not overflow
   __device__ SampleRow(float z_max, float T) {   // the same in all lanes: kept in scalar registers
     z_max = uniform(z_max);
     infinite = z_max == INFINITY;
@@ -147,7 +175,7 @@ struct SampleRow {
     c = uniform(1.4426950408889634074 / (double)T);
     top64 = uniform((double)top);
     half_top = uniform(0.5f * top);
-    step = uniform((float)fmin(6.0 * c, 3.0e38));
+    step = uniform((float)fmin(12.0 * c, 3.0e38));
   }
   __device__ static inline float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
   __device__ static inline double uniform(double x) {
@@ -156,15 +184,15 @@ struct SampleRow {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
   }
   __device__ inline float see(float z) const { return !infinite ? z : z == INFINITY ? 0.0f : -INFINITY; }
-  // The place among the bins: bin i holds place in [i, i + 1).  Ascends as z descends; from 126 on (w < 2^-42) a token
+  // The place among the bins: bin i holds place in [i, i + 1).  Ascends as z descends; from 252 on (w < 2^-42) a token
   // counts as nothing, and for NaN and -infinity no comparison holds.
   __device__ inline float place(float z) const { return fmaf(z, -0.5f, half_top) * step; }
-  __device__ static inline bool alive(float place) { return place < 126.0f; }
+  __device__ static inline bool alive(float place) { return place < 252.0f; }
   __device__ inline double log2_weight(float z) const { return ((double)z - top64) * c; }
   __device__ inline double weight(float z) const { return alive(place(z)) ? exp2_small(log2_weight(z)) : 0.0; }
-  // the weight in 2^-40: adding 2^12 leaves it in the low bits of the mantissa, rounded to nearest
+  // the weight in 2^-39: adding 2^13 leaves it in the low bits of the mantissa, rounded to nearest
   __device__ static inline uint64_t mass(double w) {
-    return __builtin_bit_cast(uint64_t, w + 4096.0) & (kSampCount - 1);
+    return __builtin_bit_cast(uint64_t, w + 8192.0) & (kSampCount - 1);
   }
 };
 
@@ -180,11 +208,11 @@ struct SampleShared {
   float red_f[kSampWaves];
   uint64_t red_u[kSampWaves];
   int red_i[kSampWaves];
-  uint32_t bound[kSampBoundBins];
-  Bins<kSampBins> row;
-  Bins<kWorkBins> work;
-  int n_list, found;
-  unsigned long long first, last;
+  union {
+    uint32_t bound[kSampBoundBins];   // while the list's bound is looked for
+    Bins<kSampBins> row;
+  };
+  int n_list, n_work, found;
 };
 
 template <int NT = kSampThreads>
@@ -253,6 +281,25 @@ __device__ __forceinline__ void sweep(const typename IN::T* row, int vocab, int 
     }
   }
 }
+// The same, token by token: f(z, i) with z = -infinity where i is not of the row.  A vector's elements go through one copy of
+// f, shifted down to the first register in turn: for the passes that few rows take, so that their code stays small.
+template <class IN, class F>
+__device__ __forceinline__ void each_token(const typename IN::T* row, int vocab, int vec0, int vec1, int step, F f) {
+  const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(typename IN::T));
+  const u32x4* base = reinterpret_cast<const u32x4*>(row - off);
+  if (vec0 >= vec1) return;
+  u32x4 next = base[vec0];
+#pragma unroll 1
+  for (int j = vec0; j < vec1; j += step) {
+    u32x4 w = next;
+    next = base[min(j + step, vec1 - 1)];
+    int i = j * IN::kVec - off;
+#pragma unroll 1
+    for (int e = 0; e < IN::kVec; ++e, ++i) {
+      f((uint32_t)i < (uint32_t)vocab ? IN::shift(w) : (IN::shift(w), -INFINITY), i);
+    }
+  }
+}
 template <class IN>
 __device__ inline int row_vectors(const typename IN::T* row, int vocab) {
   const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(typename IN::T));
@@ -260,44 +307,50 @@ __device__ inline int row_vectors(const typename IN::T* row, int vocab) {
 }
 
 // torch.argmax: NaN first, then the largest, the lowest index among equals.
-template <class IN>
-__device__ __forceinline__ int argmax_row(const typename IN::T* row, int vocab, SampleShared& sh) {
-  float best = -INFINITY;
-  int at = 0x7fffffff;
-  sweep<IN, 2>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
-#pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) {
-      const int i = i0 + e;
-      if (i < 0 || i >= vocab) continue;
-      const float v = z[e] == z[e] ? z[e] : INFINITY;
-      const bool nan = z[e] != z[e], had = best != best;
-      const bool better = at == 0x7fffffff || (nan && !had) || (!had && !nan && v > best);
-      if (better) {   // a thread's indexes ascend: the first of equals stays
-        best = z[e];
-        at = i;
-      }
-    }
-  });
-  const auto pick = [](float& v, int& i, float v2, int i2) {
+struct Best {
+  float v;
+  int i;
+  __device__ inline void pick(float v2, int i2) {
     const bool n1 = v != v, n2 = v2 != v2;
-    const bool take = n1 != n2 ? n2 : (n1 || v == v2) ? i2 < i : v2 > v;
-    if (take) {
+    if (n1 != n2 ? n2 : (n1 || v == v2) ? i2 < i : v2 > v) {
       v = v2;
       i = i2;
     }
-  };
+  }
+};
+template <int NT>
+__device__ __forceinline__ Best block_best(Best b, SampleShared& sh) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) pick(best, at, __shfl_xor(best, o), __shfl_xor(at, o));
+  for (int o = 32; o; o >>= 1) b.pick(__shfl_xor(b.v, o), __shfl_xor(b.i, o));
   if ((threadIdx.x & 63) == 0) {
-    sh.red_f[threadIdx.x >> 6] = best;
-    sh.red_i[threadIdx.x >> 6] = at;
+    sh.red_f[threadIdx.x >> 6] = b.v;
+    sh.red_i[threadIdx.x >> 6] = b.i;
   }
   __syncthreads();
-  best = sh.red_f[0];
-  at = sh.red_i[0];
-  for (int w = 1; w < kSampWaves; ++w) pick(best, at, sh.red_f[w], sh.red_i[w]);
+  b = Best{sh.red_f[0], sh.red_i[0]};
+  for (int w = 1; w < NT / kWave; ++w) b.pick(sh.red_f[w], sh.red_i[w]);
   __syncthreads();
-  return at;
+  return b;
+}
+template <class IN, int NT>
+__device__ __forceinline__ Best argmax_row(const typename IN::T* row, int vocab, int v0, int v1, SampleShared& sh) {
+  Best best{-INFINITY, 0x7fffffff};
+  sweep<IN, 2>(row, vocab, v0 + (int)threadIdx.x, v1, NT, [&](const auto& z, int i0) {
+    // a thread's indexes ascend, so only a larger logit or a first NaN changes its best; the first token always does
+    float most = z[0];
+    bool look = z[0] != z[0];
+#pragma unroll
+    for (int e = 1; e < IN::kVec; ++e) {
+      most = fmaxf(most, z[e]);
+      look |= z[e] != z[e];
+    }
+    if (look || most > best.v || best.i == 0x7fffffff) {
+#pragma unroll
+      for (int e = 0; e < IN::kVec; ++e)
+        if (i0 + e >= 0 && i0 + e < vocab) best.pick(z[e], i0 + e);
+    }
+  });
+  return block_best<NT>(best, sh);
 }
 
 // ---- the sorted list ------------------------------------------------------------
@@ -359,13 +412,25 @@ __device__ __forceinline__ void sum_list(const uint64_t* list, uint64_t* prefix,
   __syncthreads();
 }
 
-// First entry whose inclusive mass (with `base` before the list) is > target, or >= it; n if none.
-__device__ inline int first_past(const uint64_t* prefix, int n, uint64_t base, double target, bool or_equal) {
+// What a search stops at: the token of a rank (0-based), or the first whose inclusive mass passes a target.
+// Masses are whole numbers: one is > target from floor(target) + 1 on, >= target from ceil(target) on.
+struct Search {
+  bool by_rank;
+  int64_t rank;
+  uint64_t least;   // the mass from which on a search for a mass stops
+  __device__ static inline Search of_rank(int64_t rank) { return Search{true, rank, 0}; }
+  __device__ static inline Search over(double target) { return Search{false, 0, (uint64_t)fmax(target, 0.0) + 1}; }
+  __device__ static inline Search from(double target) { return Search{false, 0, (uint64_t)ceil(fmax(target, 0.0))}; }
+  __device__ inline bool past(int64_t count, uint64_t mass) const {   // of the tokens up to and with some token
+    return by_rank ? count > rank : mass >= least;
+  }
+};
+// First entry where the inclusive mass (with `base` before the list) is least or more; n if none.
+__device__ inline int first_past(const uint64_t* prefix, int n, uint64_t base, uint64_t least) {
   int lo = 0, hi = n;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    const double s = (double)(base + prefix[mid]);
-    if (or_equal ? s >= target : s > target) hi = mid;
+    if (base + prefix[mid] >= least) hi = mid;
     else lo = mid + 1;
   }
   return lo;
@@ -378,15 +443,12 @@ __device__ __forceinline__ void collect(const typename IN::T* row, int vocab, co
                                         SampleShared& sh, F take) {
   if (threadIdx.x == 0) sh.n_list = 0;
   __syncthreads();
-  sweep<IN, 2>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
-#pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) {
-      const float v = r.see(z[e]);
-      const uint64_t entry = entry_of(v, i0 + e);
-      if (take(v, entry)) {
-        const int at = atomicAdd(&sh.n_list, 1);
-        if (at < kSampList) list[at] = entry;
-      }
+  each_token<IN>(row, vocab, threadIdx.x, row_vectors<IN>(row, vocab), kSampThreads, [&](float z, int i) {
+    const float v = r.see(z);
+    const uint64_t entry = entry_of(v, i);
+    if (take(v, entry)) {
+      const int at = atomicAdd(&sh.n_list, 1);
+      if (at < kSampList) list[at] = entry;
     }
   });
   __syncthreads();
@@ -399,7 +461,7 @@ __device__ __forceinline__ int draw_from_list(const uint64_t* list, const uint64
   int kept = k > 0 ? min(k, n) : n;
   if (p < 1.0) {
     const double all = (double)(w_k == ~0ull ? prefix[kept - 1] : w_k);
-    kept = min(kept, first_past(prefix, kept, 0, p * all, true) + 1);
+    kept = min(kept, first_past(prefix, kept, 0, Search::from(p * all).least) + 1);
   }
   if (m > 0.0) {   // weights descend
     int lo = 0, hi = kept;
@@ -411,7 +473,7 @@ __device__ __forceinline__ int draw_from_list(const uint64_t* list, const uint64
     kept = lo;
   }
   kept = max(kept, 1);
-  const int at = min(first_past(prefix, kept, 0, u * (double)prefix[kept - 1], false), kept - 1);
+  const int at = min(first_past(prefix, kept, 0, Search::over(u * (double)prefix[kept - 1]).least), kept - 1);
   return (int)(uint32_t)list[at];
 }
 
@@ -421,22 +483,23 @@ __device__ inline void add_to_cell(uint64_t* cell, double w) {
   atomicAdd((unsigned long long*)cell, (unsigned long long)(SampleRow::mass(w) + kSampCount));
 }
 
-// Counts and masses of the bins, their columns summed up, by 8 threads each.
-template <int BINS, int COLS>
-__device__ __forceinline__ void sum_cells(const uint64_t* cells, Bins<BINS>& out) {
+// Counts and masses of the bins, their columns summed up, by kSampThreads / BINS threads each, 4 at most.
+template <int BINS>
+__device__ __forceinline__ void sum_cells(const uint64_t* cells, int cols, Bins<BINS>& out) {
   const int t = threadIdx.x;
-  if (t < BINS * 8) {
-    const int b = t >> 3, part = t & 7;
+  constexpr int kParts = kSampThreads / BINS < 4 ? kSampThreads / BINS : 4;
+  if (t < BINS * kParts) {
+    const int b = t / kParts, part = t % kParts;
     uint64_t mass = 0;
     uint32_t count = 0;
-#pragma unroll 1
-    for (int i = 0; i < COLS / 8; ++i) {
-      const uint64_t c = cells[b * COLS + part + 8 * i];
+#pragma unroll 4
+    for (int i = 0; i < cols / kParts; ++i) {
+      const uint64_t c = cells[b * cols + ((part + kParts * (i + b)) & (cols - 1))];
       mass += c & (kSampCount - 1);
-      count += (uint32_t)(c >> 52);
+      count += (uint32_t)(c >> 51);
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < kParts; o <<= 1) {
       mass += __shfl_xor(mass, o);
       count += __shfl_xor(count, o);
     }
@@ -483,15 +546,6 @@ __device__ __forceinline__ void before_bins(Bins<BINS>& b) {
   __syncthreads();
 }
 
-// What a search stops at: the token of a rank (0-based), or the first whose inclusive mass passes a target.
-struct Search {
-  bool by_rank, or_equal;
-  int64_t rank;
-  double target;
-  __device__ inline bool past(int64_t count, uint64_t mass) const {   // of the tokens up to and with some token
-    return by_rank ? count > rank : or_equal ? (double)mass >= target : (double)mass > target;
-  }
-};
 struct Found {
   int64_t rank;      // of the token
   int index;         // in the vocabulary
@@ -526,22 +580,19 @@ __device__ __forceinline__ void fill_bins(const typename IN::T* row, int vocab, 
   __syncthreads();
   uint64_t* mine = cells + (t & (kSampCols - 1));
   uint64_t n = 0, mass = 0;
-  sweep<IN, 1>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int) {
-#pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) {
-      const float v = r.see(z[e]), place = r.place(v);
-      if (SampleRow::alive(place)) {
-        const double w = exp2_small(r.log2_weight(v));
-        if (w >= m) {
-          n += 1;
-          mass += SampleRow::mass(w);
-        }
-        add_to_cell(&mine[(int)place * kSampCols], w);
+  each_token<IN>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](float z, int) {
+    const float v = r.see(z), place = r.place(v);
+    if (SampleRow::alive(place)) {
+      const double w = exp2_small(r.log2_weight(v));
+      if (w >= m) {
+        n += 1;
+        mass += SampleRow::mass(w);
       }
+      add_to_cell(&mine[(int)place * kSampCols], w);
     }
   });
   __syncthreads();
-  sum_cells<kSampBins, kSampCols>(cells, sh.row);
+  sum_cells(cells, kSampCols, sh.row);
   before_bins(sh.row);
   above = block_sum(n, sh.red_u);
   above_mass = block_sum(mass, sh.red_u);
@@ -550,20 +601,31 @@ __device__ __forceinline__ void fill_bins(const typename IN::T* row, int vocab, 
 // Where a search stops in the row, its bins being known.  The tokens of the bin are narrowed down, 64 ranges of their
 // order (key, then index) at a time: over the row while they are more than the list holds, then in the list, until at
 // most kSampSort are left, which are sorted.  Each turn divides the range of 64-bit numbers by 32 or more.
+// gathered: the list holds that many tokens, all of the bin among them, and stays as it is; or -1.
 template <class IN>
 __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells,
-                                            SampleShared& sh, const Search& s) {
+                                            SampleShared& sh, const Search& s, int gathered) {
+  __shared__ Bins<kWorkBins> turn_bins;
   const int t = threadIdx.x;
   uint64_t* list = cells;
-  uint64_t* work = cells + kSampList;   // [kWorkBins][kSampCols], then the sorted entries' prefix masses
-  static_assert(kWorkBins * kSampCols == kSampList, "the turns' cells take the second half");
+  uint64_t* work = cells + kSampList;   // the turns' cells; then the last entries, a copy and their prefix masses
+  constexpr int kRowCols = 128;         // a column counts up to 8191 tokens: of the whole row, and of the list
+  constexpr int kListCols = 32;
+  static_assert(kWorkBins * kRowCols == kSampList && 3 * kSampSort <= kSampList, "what the second half holds");
   const int b = bin_of_search(s, sh.row, 0, 0);
   const float from = (float)b, to = (float)(b + 1);
   int64_t base_count = sh.row.before[b];
   uint64_t base_mass = sh.row.mass_before[b];
-  int count = (int)sh.row.count[b], whole = 0;
+  int count = (int)sh.row.count[b], whole = max(gathered, 0);
+  // the range of the order that the bin takes up, a little wide: place says what is in it
   uint64_t first = 0, last = ~0ull;
-  bool listed = false, ranged = false;
+  const float upper = 2.0f * (r.half_top - from / r.step), lower = 2.0f * (r.half_top - to / r.step);
+  const float slack = 1e-5f * (fabsf(upper) + fabsf(lower) + fabsf(r.top));
+  if (upper + slack < FLT_MAX && lower - slack > -FLT_MAX) {
+    first = (uint64_t)~key_of(upper + slack) << 32;
+    last = (uint64_t)~key_of(lower - slack) << 32 | 0xffffffffull;
+  }
+  bool listed = gathered >= 0;
   const auto in = [&](float v, uint64_t e) {
     const float place = r.place(v);
     return place >= from && place < to && e >= first && e <= last;
@@ -574,68 +636,34 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
       whole = min(sh.n_list, kSampList);
       listed = true;
     }
-    if (count <= kSampSort) break;
-    if (!ranged) {   // the range that the tokens really take up
-      ranged = true;
-      unsigned long long lo = ~0ull, hi = 0;
-      if (listed) {
-        for (int i = t; i < whole; i += kSampThreads) {
-          const unsigned long long e = list[i];
-          lo = e < lo ? e : lo;
-          hi = e > hi ? e : hi;
-        }
-      } else {
-        sweep<IN, 1>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
-#pragma unroll
-          for (int e = 0; e < IN::kVec; ++e) {
-            const float v = r.see(z[e]);
-            const unsigned long long x = entry_of(v, i0 + e);
-            if (in(v, x)) {
-              lo = x < lo ? x : lo;
-              hi = x > hi ? x : hi;
-            }
-          }
-        });
-      }
-      if (t == 0) {
-        sh.first = ~0ull;
-        sh.last = 0;
-      }
-      __syncthreads();
-      atomicMin(&sh.first, lo);
-      atomicMax(&sh.last, hi);
-      __syncthreads();
-      first = sh.first;
-      last = sh.last;
-    }
-    const uint64_t range = last - first;   // at least kSampSort: the entries differ
+    if (listed && count <= kSampSort) break;
+    const uint64_t range = last - first;
     const int shift = max(0, 58 - (int)__builtin_clzll(range | 1));
-    for (int i = t; i < kSampList; i += kSampThreads) work[i] = 0;
+    const int cols = listed ? kListCols : kRowCols;
+    for (int i = t; i < kWorkBins * cols; i += kSampThreads) work[i] = 0;
     __syncthreads();
-    uint64_t* mine = work + (t & (kSampCols - 1));
+    uint64_t* mine = work + (t & (cols - 1));
     if (listed) {
 #pragma unroll 1
       for (int i = t; i < whole; i += kSampThreads) {
         const uint64_t e = list[i];
-        if (e >= first && e <= last) add_to_cell(&mine[(int)((e - first) >> shift) * kSampCols], r.weight(logit_of(e)));
+        const float v = logit_of(e);
+        if (in(v, e)) add_to_cell(&mine[(int)((e - first) >> shift) * cols], r.weight(v));
       }
     } else {
-      sweep<IN, 1>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](const auto& z, int i0) {
-#pragma unroll
-        for (int e = 0; e < IN::kVec; ++e) {
-          const float v = r.see(z[e]);
-          const uint64_t x = entry_of(v, i0 + e);
-          if (in(v, x)) add_to_cell(&mine[(int)((x - first) >> shift) * kSampCols], r.weight(v));
-        }
+      each_token<IN>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](float z, int i) {
+        const float v = r.see(z);
+        const uint64_t x = entry_of(v, i);
+        if (in(v, x)) add_to_cell(&mine[(int)((x - first) >> shift) * cols], r.weight(v));
       });
     }
     __syncthreads();
-    sum_cells<kWorkBins, kSampCols>(work, sh.work);
-    before_bins(sh.work);
-    const int w = bin_of_search(s, sh.work, base_count, base_mass);
-    base_count += sh.work.before[w];
-    base_mass += sh.work.mass_before[w];
-    count = (int)sh.work.count[w];
+    sum_cells(work, cols, turn_bins);
+    before_bins(turn_bins);
+    const int w = bin_of_search(s, turn_bins, base_count, base_mass);
+    base_count += turn_bins.before[w];
+    base_mass += turn_bins.mass_before[w];
+    count = (int)turn_bins.count[w];
     first += (uint64_t)w << shift;
     const uint64_t end = first + ((1ull << shift) - 1);
     last = end < last ? end : last;
@@ -646,56 +674,123 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
     }
     __syncthreads();   // the next turn writes the bins
   }
-  // the entries in the range go to the work half
   __syncthreads();   // every thread has read the list's length
-  if (t == 0) sh.n_list = 0;
+  if (t == 0) sh.n_work = 0;
   __syncthreads();
   for (int i = t; i < whole; i += kSampThreads) {
     const uint64_t e = list[i];
-    if (e >= first && e <= last) {
-      const int at = atomicAdd(&sh.n_list, 1);
+    if (in(logit_of(e), e)) {
+      const int at = atomicAdd(&sh.n_work, 1);
       if (at < kSampSort) work[at] = e;
     }
   }
   __syncthreads();
-  const int n = max(1, min(sh.n_list, kSampSort));
-  sort_small(work, list, n);
-  sum_list(work, list, n, r, sh);
-  int at = s.by_rank ? (int)(s.rank - base_count) : first_past(list, n, base_mass, s.target, s.or_equal);
+  const int n = max(1, min(sh.n_work, kSampSort));
+  uint64_t* prefix = work + 2 * kSampSort;
+  sort_small(work, work + kSampSort, n);
+  sum_list(work, prefix, n, r, sh);
+  int at = s.by_rank ? (int)(s.rank - base_count) : first_past(prefix, n, base_mass, s.least);
   at = max(min(at, n - 1), 0);
-  const Found f{base_count + at, (int)(uint32_t)work[at], base_mass + list[at]};
-  __syncthreads();   // both halves are written again
+  const Found f{base_count + at, (int)(uint32_t)work[at], base_mass + prefix[at]};
+  __syncthreads();   // the work half is written again
   return f;
 }
 
-// The answer of a row whose bins are in sh.row.
+// Whether what top-p can keep is few enough to be sorted at once, and the bin it ends in at the latest (w_most: the most
+// that top-k can have left it).
+__device__ __forceinline__ bool sort_whole(const SampleSettings& set, const Bins<kSampBins>& bins, double w_most, int& end) {
+  if (!(set.p < 1.0)) return false;
+  end = bin_of_search(Search::from(set.p * w_most), bins, 0, 0);
+  return (int64_t)bins.before[end] + bins.count[end] <= kSampWhole;
+}
+
+// The places that a row's searches can end in, from its bins: the bin where top-k ends, those where top-p can end
+// whatever top-k keeps of its bin, and those where the number can fall.
+struct Needed {
+  float from[3], to[3];
+  __device__ inline void range(int i, int b0, int b1) {
+    from[i] = (float)b0;
+    to[i] = (float)(b1 + 1);
+  }
+  __device__ inline bool has(float place) const {
+    return (place >= from[0] && place < to[0]) || (place >= from[1] && place < to[1]) || (place >= from[2] && place < to[2]);
+  }
+  __device__ __forceinline__ Needed(const SampleSettings& set, const Bins<kSampBins>& bins, uint64_t above,
+                                    uint64_t above_mass) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) range(i, -1, -2);   // nothing
+    const int64_t total = (int64_t)bins.before[kSampBins - 1] + bins.count[kSampBins - 1];
+    uint64_t lo = bins.mass_before[kSampBins - 1] + bins.mass[kSampBins - 1], hi = lo;   // the mass of what is kept
+    if (set.k > 0 && set.k < total) {
+      const int b = bin_of_search(Search::of_rank(set.k - 1), bins, 0, 0);
+      range(0, b, b);
+      lo = bins.mass_before[b];
+      hi = lo + bins.mass[b];
+    }
+    int end;
+    if (sort_whole(set, bins, (double)hi, end)) {
+      range(1, 0, end);
+      return;
+    }
+    if (set.p < 1.0) {
+      const int b = bin_of_search(Search::from(set.p * (double)lo), bins, 0, 0);
+      range(1, b, end);
+      const uint64_t through = bins.mass_before[end] + bins.mass[end];
+      lo = bins.mass_before[b] < lo ? bins.mass_before[b] : lo;
+      hi = through < hi ? through : hi;
+    }
+    if (set.m > 0.0 && above > 0) {
+      lo = above_mass < lo ? above_mass : lo;
+      hi = above_mass < hi ? above_mass : hi;
+    }
+    const bool none = set.m > 0.0 && above == 0;   // the first token alone
+    const int b0 = bin_of_search(none ? Search::of_rank(0) : Search::over((double)set.u * (double)lo), bins, 0, 0);
+    const int b1 = hi == lo ? b0 : bin_of_search(Search::over((double)set.u * (double)hi), bins, 0, 0);
+    range(2, b0, none ? b0 : b1);
+  }
+};
+
+// The answer of a row whose bins are in sh.row.  gathered: tokens in the list (Needed's), or -1.
 template <class IN>
 __device__ __forceinline__ int draw_from_bins(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells,
                                               SampleShared& sh, const SampleSettings& set, uint64_t above,
-                                              uint64_t above_mass) {
+                                              uint64_t above_mass, int gathered) {
   const int64_t total = (int64_t)sh.row.before[kSampBins - 1] + sh.row.count[kSampBins - 1];
   const uint64_t total_mass = sh.row.mass_before[kSampBins - 1] + sh.row.mass[kSampBins - 1];
   int64_t kept = total;
   uint64_t kept_mass = total_mass, w_k = total_mass;
+  double w_most = (double)total_mass;
   int answer = 0;
 #pragma unroll 1
   for (int stage = 0; stage < 4; ++stage) {   // what top-k keeps, what top-p keeps, the number, the last that is kept
-    Search s{true, false, 0, 0.0};
+    Search s = Search::of_rank(0);
     if (stage == 0) {
       if (!(set.k > 0 && set.k < total)) continue;
       s.rank = set.k - 1;
+      const int b = bin_of_search(s, sh.row, 0, 0);
+      w_most = (double)(sh.row.mass_before[b] + sh.row.mass[b]);
     } else if (stage == 1) {
       if (!(set.p < 1.0)) continue;
-      s = Search{false, true, 0, set.p * (double)w_k};
-      const int b = bin_of_search(s, sh.row, 0, 0);
-      if ((int64_t)sh.row.before[b] + sh.row.count[b] <= kSampWhole) {   // all that can be kept, at once
-        const float to = (float)(b + 1);
-        collect<IN>(row, vocab, r, cells, sh, [&](float v, uint64_t) { return r.place(v) < to; });
-        const int n = max(1, min(sh.n_list, kSampList));
-        sort_list(cells, cells + kSampList, n);
-        sum_list(cells, cells + kSampList, n, r, sh);
+      s = Search::from(set.p * (double)w_k);
+      int end;
+      if (sort_whole(set, sh.row, w_most, end)) {
+        const float to = (float)(end + 1);
+        if (gathered < 0) {
+          collect<IN>(row, vocab, r, cells, sh, [&](float v, uint64_t) { return r.place(v) < to; });
+        } else {   // the list without what is only top-k's
+          uint64_t* work = cells + kSampList;
+          if (threadIdx.x == 0) sh.n_list = 0;
+          __syncthreads();
+          for (int i = threadIdx.x; i < gathered; i += kSampThreads)
+            if (r.place(logit_of(cells[i])) < to) work[atomicAdd(&sh.n_list, 1)] = cells[i];
+          __syncthreads();
+          cells = work;
+        }
+        const int n = max(1, min(sh.n_list, kSampWhole));
+        sort_list(cells, cells + kSampWhole, n);
+        sum_list(cells, cells + kSampWhole, n, r, sh);
         const int k = set.k > 0 ? (int)(kept < n ? kept : n) : 0;
-        return draw_from_list(cells, cells + kSampList, n, k, set.p, set.m, set.u, w_k, r);
+        return draw_from_list(cells, cells + kSampWhole, n, k, set.p, set.m, set.u, w_k, r);
       }
     } else if (stage == 2) {
       if (set.m > 0.0 && (int64_t)above < kept) {
@@ -703,11 +798,12 @@ __device__ __forceinline__ int draw_from_bins(const typename IN::T* row, int voc
         kept_mass = above_mass;
       }
       // where nothing is likely enough the first token alone is kept
-      if (!(set.m > 0.0 && above == 0)) s = Search{false, false, 0, (double)set.u * (double)kept_mass};
+      if (!(set.m > 0.0 && above == 0)) s = Search::over((double)set.u * (double)kept_mass);
     } else {
       s.rank = kept - 1;   // a number of 1 or more
+      gathered = -1;
     }
-    const Found f = search_row<IN>(row, vocab, r, cells, sh, s);
+    const Found f = search_row<IN>(row, vocab, r, cells, sh, s, gathered);
     if (stage == 0) {
       kept = set.k;
       w_k = kept_mass = f.through;
@@ -794,7 +890,7 @@ sample_kernel(SampleArgs a) {
   }
   int token = -1;
   if (top == -INFINITY) {
-    token = argmax_row<IN>(row, a.vocab, sh);
+    token = argmax_row<IN, kSampThreads>(row, a.vocab, 0, row_vectors<IN>(row, a.vocab), sh).i;
   } else {
     const SampleRow r(top, set.T);
     mine = r.see(mine);
@@ -812,7 +908,7 @@ sample_kernel(SampleArgs a) {
     if (token < 0) {
       uint64_t above, above_mass;
       fill_bins<IN>(row, a.vocab, r, set.m, cells, sh, above, above_mass);
-      token = draw_from_bins<IN>(row, a.vocab, r, cells, sh, set, above, above_mass);
+      token = draw_from_bins<IN>(row, a.vocab, r, cells, sh, set, above, above_mass, -1);
     }
   }
   if (t == 0) a.out[b] = token;
@@ -832,60 +928,109 @@ sample_max_kernel(SampleArgs a) {
   const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
   int v0, v1;
   chunk_range(row_vectors<IN>(row, a.vocab), a.chunks, c, v0, v1);
+  float* maxima = a.maxima + (int64_t)b * a.chunks * a.per;
+  if (c == 0 && t == 0) a.n_list[b] = 0;
+  if (SampleSettings(a, b).greedy()) {
+    __shared__ SampleShared sh;
+    const Best best = argmax_row<IN, kChunkThreads>(row, a.vocab, v0, v1, sh);
+    if (t == 0) {
+      maxima[c] = best.v;
+      a.best[(int64_t)b * a.chunks + c] = best.i;
+    }
+    return;
+  }
   float mine = -INFINITY;
   sweep<IN, 4>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int) {
 #pragma unroll
     for (int e = 0; e < IN::kVec; ++e) mine = fmaxf(mine, z[e]);
   });
-  a.maxima[((int64_t)b * a.chunks + c) * kChunkThreads + t] = mine;
-  if (c == 0 && t == 0) a.n_list[b] = 0;
+  const int group = kChunkThreads / a.per;   // 1 .. 32 neighbours
+  for (int o = 1; o < group; o <<= 1) mine = fmaxf(mine, __shfl_xor(mine, o));
+  if ((t & (group - 1)) == 0) maxima[c * a.per + t / group] = mine;
+}
+
+// The maxima of a row in registers, and the largest.
+template <int NT>
+struct RowMaxima {
+  static constexpr int kMine = (kMaxima + NT - 1) / NT;
+  float z[kMine];
+  __device__ __forceinline__ float load(const SampleArgs& a, int b, SampleShared& sh) {
+    const int n = a.chunks * a.per;
+    const float* from = a.maxima + (int64_t)b * n;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = (int)threadIdx.x + i * NT;
+      z[i] = j < n ? from[j] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) top = fmaxf(top, z[i]);
+    return block_max_f<NT>(top, sh.red_f);
+  }
+};
+
+// The chunk's tokens that `take` accepts, through LDS to the row's list.
+template <class IN, class F>
+__device__ __forceinline__ void hand_over(const SampleArgs& a, int b, const typename IN::T* row, int v0, int v1,
+                                          const SampleRow& r, uint64_t* list, SampleShared& sh, F take) {
+  const int t = threadIdx.x;
+  if (t == 0) sh.n_list = 0;
+  __syncthreads();
+  sweep<IN, 1>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int i0) {
+#pragma unroll
+    for (int e = 0; e < IN::kVec; ++e) {
+      const float v = r.see(z[e]);
+      if (take(v)) {
+        const int at = atomicAdd(&sh.n_list, 1);
+        if (at < kChunkList) list[at] = entry_of(v, i0 + e);
+      }
+    }
+  });
+  __syncthreads();
+  // more than fit here: a number that no list holds
+  const int n = sh.n_list;
+  if (t == 0) sh.n_work = (int)min(atomicAdd(&a.n_list[b], n <= kChunkList ? (uint32_t)n : 1u << 20), 1u << 24);
+  __syncthreads();
+  const int at = sh.n_work;
+  if (n > kChunkList || at + n > a.list_cap) return;
+  for (int i = t; i < n; i += kChunkThreads) a.list[(int64_t)b * a.list_cap + at + i] = list[i];
 }
 
 template <class IN>
 __global__ void __launch_bounds__(kChunkThreads)
 sample_chunk_kernel(SampleArgs a) {
   __shared__ uint64_t cells[kSampBins * kChunkCols];
+  static_assert(kSampBins * kChunkCols >= kChunkList, "the list takes the cells' place");
   __shared__ SampleShared sh;
   const int b = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
   const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
   const SampleSettings set(a, b);
   if (set.greedy()) return;
-  const float* maxima = a.maxima + (int64_t)b * a.chunks * kChunkThreads;
-  float mine = -INFINITY;
-  for (int i = t; i < a.chunks * kChunkThreads; i += kChunkThreads) mine = fmaxf(mine, maxima[i]);
-  const float top = block_max_f<kChunkThreads>(mine, sh.red_f);
+  RowMaxima<kChunkThreads> maxima;
+  const float top = maxima.load(a, b, sh);
   if (top == -INFINITY) return;
   const SampleRow r(top, set.T);
   int v0, v1;
   chunk_range(row_vectors<IN>(row, a.vocab), a.chunks, c, v0, v1);
   if (set.by_list()) {
     const float bound = list_bound<kChunkThreads>(set, r, sh, [&](auto f) {
-      for (int i = t; i < a.chunks * kChunkThreads; i += kChunkThreads) f(r.see(maxima[i]));
-    });
-    uint64_t* list = a.list + (int64_t)b * kChunkList;
-    sweep<IN, 2>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int i0) {
 #pragma unroll
-      for (int e = 0; e < IN::kVec; ++e) {
-        const float v = r.see(z[e]);
-        if (v >= bound) {
-          const uint32_t at = atomicAdd(&a.n_list[b], 1u);
-          if (at < (uint32_t)kChunkList) list[at] = entry_of(v, i0 + e);
-        }
-      }
+      for (int i = 0; i < RowMaxima<kChunkThreads>::kMine; ++i) f(r.see(maxima.z[i]));
     });
+    hand_over<IN>(a, b, row, v0, v1, r, cells, sh, [&](float v) { return v >= bound; });
     return;
   }
   for (int i = t; i < kSampBins * kChunkCols; i += kChunkThreads) cells[i] = 0;
   __syncthreads();
   uint64_t* own = cells + (t & (kChunkCols - 1));
   uint64_t above = 0, above_mass = 0;
-  sweep<IN, 2>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int) {
+  sweep<IN, 1>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int) {
 #pragma unroll
     for (int e = 0; e < IN::kVec; ++e) {
       const float v = r.see(z[e]), place = r.place(v);
       if (SampleRow::alive(place)) {
         const double w = exp2_small(r.log2_weight(v));
-        if (w >= set.m) {
+        if (set.m > 0.0 && w >= set.m) {
           above += 1;
           above_mass += SampleRow::mass(w);
         }
@@ -897,25 +1042,77 @@ sample_chunk_kernel(SampleArgs a) {
   above_mass = block_sum<kChunkThreads>(above_mass, sh.red_u);
   const int64_t at = (int64_t)b * a.chunks + c;
   {
-    const int bin = t >> 1, part = t & 1;
+    static_assert(kSampBins == kChunkThreads, "a thread sums up a bin");
     uint64_t mass = 0;
     uint32_t count = 0;
-    for (int i = 0; i < kChunkCols / 2; ++i) {
-      const uint64_t w = cells[bin * kChunkCols + 2 * i + part];
+#pragma unroll
+    for (int i = 0; i < kChunkCols; ++i) {   // every thread from a column of its own on: no bank conflicts
+      const uint64_t w = cells[t * kChunkCols + ((i + t) & (kChunkCols - 1))];
       mass += w & (kSampCount - 1);
-      count += (uint32_t)(w >> 52);
+      count += (uint32_t)(w >> 51);
     }
-    mass += __shfl_xor(mass, 1);
-    count += __shfl_xor(count, 1);
-    if (part == 0) {
-      a.bin_mass[at * kSampBins + bin] = mass;
-      a.bin_count[at * kSampBins + bin] = count;
-    }
+    a.bin_mass[at * kSampBins + t] = mass;
+    a.bin_count[at * kSampBins + t] = count;
   }
   if (t == 0) {
     a.above[at] = (uint32_t)above;
     a.above_mass[at] = above_mass;
   }
+}
+
+// The bins of a row from those of its chunks, by kSampBins threads or more.
+__device__ __forceinline__ void row_bins(const SampleArgs& a, int b, SampleShared& sh, uint64_t& above, uint64_t& above_mass) {
+  const int t = threadIdx.x;
+  const int64_t at = (int64_t)b * a.chunks;
+  if (t < kSampBins) {
+    uint64_t mass = 0;
+    uint32_t count = 0;
+#pragma unroll 16
+    for (int c = 0; c < a.chunks; ++c) {
+      mass += a.bin_mass[(at + c) * kSampBins + t];
+      count += a.bin_count[(at + c) * kSampBins + t];
+    }
+    sh.row.mass[t] = mass;
+    sh.row.count[t] = count;
+  }
+  above = above_mass = 0;
+#pragma unroll 8
+  for (int c = 0; c < a.chunks; ++c) {
+    above += a.above[at + c];
+    above_mass += a.above_mass[at + c];
+  }
+  __syncthreads();
+  before_bins(sh.row);
+}
+
+template <class IN>
+__global__ void __launch_bounds__(kChunkThreads)
+sample_gather_kernel(SampleArgs a) {
+  __shared__ uint64_t list[kChunkList];
+  __shared__ SampleShared sh;
+  const int b = blockIdx.y, c = blockIdx.x;
+  const SampleSettings set(a, b);
+  if (set.greedy() || set.by_list()) return;
+  const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
+  RowMaxima<kChunkThreads> maxima;
+  const float top = maxima.load(a, b, sh);
+  if (top == -INFINITY) return;
+  const SampleRow r(top, set.T);
+  uint64_t above, above_mass;
+  row_bins(a, b, sh, above, above_mass);
+  if (c == 0) {   // for the workgroup that finishes the row
+    const int t = threadIdx.x;
+    a.row_mass[(int64_t)b * (kSampBins + 2) + t] = sh.row.mass[t];
+    a.row_count[(int64_t)b * kSampBins + t] = sh.row.count[t];
+    if (t == 0) {
+      a.row_mass[(int64_t)b * (kSampBins + 2) + kSampBins] = above_mass;
+      a.row_mass[(int64_t)b * (kSampBins + 2) + kSampBins + 1] = above;
+    }
+  }
+  const Needed needed(set, sh.row, above, above_mass);
+  int v0, v1;
+  chunk_range(row_vectors<IN>(row, a.vocab), a.chunks, c, v0, v1);
+  hand_over<IN>(a, b, row, v0, v1, r, list, sh, [&](float v) { return needed.has(r.place(v)); });
 }
 
 template <class IN>
@@ -926,88 +1123,96 @@ sample_finish_kernel(SampleArgs a) {
   const int t = threadIdx.x, b = blockIdx.x;
   const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
   const SampleSettings set(a, b);
-  const float* maxima = a.maxima + (int64_t)b * a.chunks * kChunkThreads;
-  float top = -INFINITY;
-  if (!set.greedy()) {
-    for (int i = t; i < a.chunks * kChunkThreads; i += kSampThreads) top = fmaxf(top, maxima[i]);
-    top = block_max_f(top, sh.red_f);
+  if (set.greedy()) {
+    Best best{-INFINITY, 0x7fffffff};
+    if (t < a.chunks) best = Best{a.maxima[(int64_t)b * a.chunks * a.per + t], a.best[(int64_t)b * a.chunks + t]};
+    best = block_best<kSampThreads>(best, sh);
+    if (t == 0) a.out[b] = best.i;
+    return;
   }
+  RowMaxima<kSampThreads> maxima;
+  const float top = maxima.load(a, b, sh);
   int token;
   if (top == -INFINITY) {
-    token = argmax_row<IN>(row, a.vocab, sh);
+    token = argmax_row<IN, kSampThreads>(row, a.vocab, 0, row_vectors<IN>(row, a.vocab), sh).i;
   } else {
     const SampleRow r(top, set.T);
-    const uint32_t listed = set.by_list() ? a.n_list[b] : ~0u;
-    if (listed <= (uint32_t)kChunkList) {
-      const int n = (int)listed;
-      for (int i = t; i < n; i += kSampThreads) cells[i] = a.list[(int64_t)b * kChunkList + i];
-      __syncthreads();
+    const uint32_t listed = a.n_list[b];
+    const int n = listed <= (uint32_t)a.list_cap ? (int)listed : -1;
+    for (int i = t; i < n; i += kSampThreads) cells[i] = a.list[(int64_t)b * a.list_cap + i];
+    __syncthreads();
+    if (set.by_list() && n >= 0) {
       sort_list(cells, cells + kSampList, n);
       sum_list(cells, cells + kSampList, n, r, sh);
       token = draw_from_list(cells, cells + kSampList, n, set.k, set.p, set.m, set.u, ~0ull, r);
     } else {
-      uint64_t above = 0, above_mass = 0;
-      if (set.by_list()) {   // more than the chunks could hand over
+      uint64_t above, above_mass;
+      if (set.by_list()) {   // more than could be handed over
         fill_bins<IN>(row, a.vocab, r, set.m, cells, sh, above, above_mass);
       } else {
+        const uint64_t* mass = a.row_mass + (int64_t)b * (kSampBins + 2);
         if (t < kSampBins) {
-          uint64_t mass = 0;
-          uint32_t count = 0;
-          for (int c = 0; c < a.chunks; ++c) {
-            mass += a.bin_mass[((int64_t)b * a.chunks + c) * kSampBins + t];
-            count += a.bin_count[((int64_t)b * a.chunks + c) * kSampBins + t];
-          }
-          sh.row.mass[t] = mass;
-          sh.row.count[t] = count;
+          sh.row.mass[t] = mass[t];
+          sh.row.count[t] = a.row_count[(int64_t)b * kSampBins + t];
         }
-        for (int c = 0; c < a.chunks; ++c) {
-          above += a.above[(int64_t)b * a.chunks + c];
-          above_mass += a.above_mass[(int64_t)b * a.chunks + c];
-        }
+        above_mass = mass[kSampBins];
+        above = mass[kSampBins + 1];
         __syncthreads();
         before_bins(sh.row);
       }
-      token = draw_from_bins<IN>(row, a.vocab, r, cells, sh, set, above, above_mass);
+      token = draw_from_bins<IN>(row, a.vocab, r, cells, sh, set, above, above_mass, n);
     }
   }
   if (t == 0) a.out[b] = token;
 }
 
-// Chunks of a row, 0: one workgroup takes it whole.
-static int sample_chunks(int rows, int vocab) {
-  if (vocab < 16384) return 0;
-  int c = 1024 / rows;
-  c = c < 1 ? 1 : c > 32 ? 32 : c;
+// How a call's rows are cut.  chunks 0: one workgroup takes a row whole.
+struct SamplePlan {
+  int chunks, per, list_cap;
+  int64_t words;   // of 8 bytes, of the workspace
+};
+static SamplePlan sample_plan(int rows, int vocab) {
+  if (vocab < 16384) return SamplePlan{0, 0, 0, 0};
+  int c = 2048 / rows;
+  c = c < 1 ? 1 : c > 16 ? 16 : c;
   const int most = vocab / 2048, least = (vocab + kChunkMost - 1) / kChunkMost;
   c = c > most ? most : c;
-  return c < least ? least : c;
-}
-
-// 8-byte words of the split form's workspace.
-static int64_t sample_words(int rows, int chunks) {
-  return (int64_t)rows * (chunks * (kChunkThreads / 2 + kSampBins + kSampBins / 2 + 2) + kChunkList + 1);
+  c = c < least ? least : c;
+  SamplePlan p{c, kChunkThreads, rows <= 512 ? kSampList : rows <= 4096 ? kSampList / 4 : kSampList / 16, 0};
+  while (p.per * c > kMaxima && p.per > 8) p.per /= 2;
+  p.words = (int64_t)rows * ((int64_t)c * (p.per / 2 + kSampBins + kSampBins / 2 + 2) + p.list_cap + 1 +
+                              kSampBins + 2 + kSampBins / 2);
+  return p;
 }
 
 template <class IN>
-static int sample_launch(SampleArgs a, uint64_t* ws, hipStream_t s) {
+static int sample_launch(SampleArgs a, const SamplePlan& p, uint64_t* ws, hipStream_t s) {
   constexpr size_t lds = (size_t)kSampBins * kSampCols * sizeof(uint64_t);
   static_assert((size_t)kSampList * 16 == lds, "list and prefix take the bins' place");
-  if (a.chunks == 0) {
+  if (p.chunks == 0) {
     TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_kernel<IN>>(lds)));
     hipLaunchKernelGGL(sample_kernel<IN>, dim3(a.rows), dim3(kSampThreads), lds, s, a);
     return (int)hipGetLastError();
   }
-  const int64_t n = (int64_t)a.rows * a.chunks;
+  const int64_t n = (int64_t)a.rows * p.chunks;
+  a.chunks = p.chunks;
+  a.per = p.per;
+  a.list_cap = p.list_cap;
   a.bin_mass = ws;
   a.list = a.bin_mass + n * kSampBins;
-  a.above_mass = a.list + (int64_t)a.rows * kChunkList;
-  a.maxima = reinterpret_cast<float*>(a.above_mass + n);
-  a.bin_count = reinterpret_cast<uint32_t*>(a.maxima + n * kChunkThreads);
-  a.above = a.bin_count + n * kSampBins;
-  a.n_list = a.above + n;
+  a.above_mass = a.list + (int64_t)a.rows * p.list_cap;
+  a.row_mass = a.above_mass + n;
+  a.maxima = reinterpret_cast<float*>(a.row_mass + (int64_t)a.rows * (kSampBins + 2));
+  a.bin_count = reinterpret_cast<uint32_t*>(a.maxima + n * p.per);
+  a.row_count = a.bin_count + n * kSampBins;
+  a.above = a.row_count + (int64_t)a.rows * kSampBins;
+  a.best = reinterpret_cast<int32_t*>(a.above + n);
+  a.n_list = reinterpret_cast<uint32_t*>(a.best + n);
   TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_finish_kernel<IN>>(lds)));
-  hipLaunchKernelGGL(sample_max_kernel<IN>, dim3(a.chunks, a.rows), dim3(kChunkThreads), 0, s, a);
-  hipLaunchKernelGGL(sample_chunk_kernel<IN>, dim3(a.chunks, a.rows), dim3(kChunkThreads), 0, s, a);
+  const dim3 grid(p.chunks, a.rows), block(kChunkThreads);
+  hipLaunchKernelGGL(sample_max_kernel<IN>, grid, block, 0, s, a);
+  hipLaunchKernelGGL(sample_chunk_kernel<IN>, grid, block, 0, s, a);
+  hipLaunchKernelGGL(sample_gather_kernel<IN>, grid, block, 0, s, a);
   hipLaunchKernelGGL(sample_finish_kernel<IN>, dim3(a.rows), dim3(kSampThreads), lds, s, a);
   return (int)hipGetLastError();
 }
@@ -1018,8 +1223,7 @@ using namespace tq;
 
 extern "C" int64_t tq_sample_workspace_elems(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kSampMaxVocab) return 0;
-  const int c = sample_chunks(rows, vocab);
-  return c ? sample_words(rows, c) : 0;
+  return sample_plan(rows, vocab).words;
 }
 
 extern "C" int tq_sample_tokens(const void* logits, int64_t logits_stride, int dtype, int rows, int vocab,
@@ -1039,12 +1243,12 @@ extern "C" int tq_sample_tokens(const void* logits, int64_t logits_stride, int d
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
   a.temperature0 = temperature_all; a.top_k0 = top_k_all; a.top_p0 = top_p_all; a.min_p0 = min_p_all;
   a.out = tokens; a.rows = rows; a.vocab = vocab;
-  a.chunks = sample_chunks(rows, vocab);
-  if (a.chunks && (!workspace || workspace_elems < sample_words(rows, a.chunks))) return TQ_ERR_WORKSPACE;
+  const SamplePlan p = sample_plan(rows, vocab);
+  if (p.chunks && (!workspace || workspace_elems < p.words)) return TQ_ERR_WORKSPACE;
   uint64_t* ws = reinterpret_cast<uint64_t*>(workspace);
   if (reinterpret_cast<uintptr_t>(ws) & 7u) return TQ_ERR_ALIGN;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == TQ_DTYPE_BF16) return sample_launch<H16In<Bf16>>(a, ws, s);
-  if (dtype == TQ_DTYPE_FP16) return sample_launch<H16In<Fp16>>(a, ws, s);
-  return sample_launch<F32In>(a, ws, s);
+  if (dtype == TQ_DTYPE_BF16) return sample_launch<H16In<Bf16>>(a, p, ws, s);
+  if (dtype == TQ_DTYPE_FP16) return sample_launch<H16In<Fp16>>(a, p, ws, s);
+  return sample_launch<F32In>(a, p, ws, s);
 }
