@@ -158,10 +158,13 @@ struct UnitInfo {
   bool ok;   // the page is one of the cache's
 };
 
-__device__ inline int64_t kv8_page(const Kv8Args& a, const int32_t* row, int unit, bool inside, bool* ok) {
-  const int32_t page = inside ? row[unit >> a.unit_shift] : -1;
-  *ok = (uint32_t)page < (uint32_t)a.pages;
-  return *ok ? page : 0;
+// The table's entry for a unit below the key limit (-1 beyond), and whether it is a page of the cache; page 0 stands in.
+__device__ inline int32_t kv8_entry(const Kv8Args& a, const int32_t* row, int unit, int limit) {
+  return unit * 16 < limit ? row[unit >> a.unit_shift] : -1;
+}
+__device__ inline int64_t kv8_page(const Kv8Args& a, int32_t entry, bool* ok) {
+  *ok = (uint32_t)entry < (uint32_t)a.pages;
+  return *ok ? entry : 0;
 }
 
 // Running softmax of one query row per lane column: M, the sum (of this lane's units), and what each tile does to them.
@@ -169,11 +172,20 @@ struct Softmax {
   float M, l;
 };
 
+// A value scale as the softmax takes it: log2 and reciprocal of what P is multiplied with.
+struct ValueScale {
+  float log, inv;
+  __device__ inline explicit ValueScale(float vs) {
+    const float t = vs > 0.0f ? vs : 0.00390625f;
+    log = __builtin_amdgcn_logf(t);
+    inv = __builtin_amdgcn_rcpf(t);
+  }
+};
+
 // The tile's probabilities as the P operands, from the raw products; returns the factor of what was summed before.
 // nv: how many of the lane's 16 keys its row sees (the lane's key index is 4 m + v).
-__device__ inline float softmax_tile(v4f (&s)[4], int nv, float f, float vs, Softmax& sm, v4i (&p)[2]) {
-  const float t = vs > 0.0f ? vs : 0.00390625f;
-  const float lv = __builtin_amdgcn_logf(t);
+__device__ inline float softmax_tile(v4f (&s)[4], int nv, float f, const ValueScale& vs, Softmax& sm, v4i (&p)[2]) {
+  const float lv = vs.log;
   const bool whole = __all(nv == 16);
   if (!whole) {
 #pragma unroll
@@ -203,7 +215,7 @@ __device__ inline float softmax_tile(v4f (&s)[4], int nv, float f, float vs, Sof
   }
   const float alpha = __builtin_amdgcn_exp2f(sm.M - ref);
   sm.M = M;
-  sm.l = fmaf(sm.l, alpha, sum / t);
+  sm.l = fmaf(sm.l, alpha, sum * vs.inv);
   return alpha;
 }
 
@@ -244,12 +256,14 @@ kv8_split_kernel(Kv8Args a) {
   for (int d = 0; d < DB; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
   Softmax sm{-INFINITY, 0.0f};
 
-  for (int base = key0 + wave * kKv8Tile; base < key1; base += NW * kKv8Tile) {
+  // a tile's table entries are loaded a tile ahead: the codes' loads wait for nothing else
+  int base = key0 + wave * kKv8Tile;
+  int32_t ek = kv8_entry(a, row, (base >> 4) + (c >> 2), key1), ev = kv8_entry(a, row, (base >> 4) + g, key1);
+  for (; base < key1; base += NW * kKv8Tile) {
     // units: of the key this lane loads as an A row, and of the keys whose scores it holds (and whose values it loads)
     const int uk = (base >> 4) + (c >> 2), uv = (base >> 4) + g;
     bool okk, okv;
-    const int64_t pk = kv8_page(a, row, uk, uk * 16 < key1, &okk);
-    const int64_t pv = kv8_page(a, row, uv, uv * 16 < key1, &okv);
+    const int64_t pk = kv8_page(a, ek, &okk), pv = kv8_page(a, ev, &okv);
     const int8_t* kp = a.k + (pk * a.kv_heads + h) * a.head_bytes + (uk & (a.units - 1)) * (16 * D) + (c & 3) * D + g * 16;
     const int8_t* vp = a.v + (pv * a.kv_heads + h) * a.head_bytes + (uv & (a.units - 1)) * (16 * D) + c * 16;
     u32x4 kw[4][HF], vw[DB];
@@ -261,6 +275,8 @@ kv8_split_kernel(Kv8Args a) {
     float ks = a.ks[cell], vs = a.vs[cell];
 #pragma unroll
     for (int d = 0; d < DB; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + d * 256);
+    ek = kv8_entry(a, row, uk + NW * (kKv8Tile / 16), key1);
+    ev = kv8_entry(a, row, uv + NW * (kKv8Tile / 16), key1);
     const int nv = okv ? min(max(min(seen, key1) - uv * 16, 0), 16) : 0;
     if (nv == 0) ks = 0.0f, vs = 1.0f;   // whatever the scales of a page that is not there are
 
@@ -276,7 +292,7 @@ kv8_split_kernel(Kv8Args a) {
     }
     v4i p[2];
     const float before = sm.M;
-    const float alpha = softmax_tile(s, nv, qr.factor * ks, vs, sm, p);
+    const float alpha = softmax_tile(s, nv, qr.factor * ks, ValueScale(vs), sm, p);
     if (__any(sm.M != before)) {
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -381,16 +397,16 @@ kv8_block_kernel(Kv8Args a) {
     for (int d = 0; d < DB; ++d) o[x][d] = v4f{0.f, 0.f, 0.f, 0.f};
   }
 
-  // this wave's quarter of a tile: key block m = wave, and DB / 4 blocks of the values
+  // this wave's quarter of a tile: key block m = wave, and DB / 4 blocks of the values; table entries a tile ahead
   constexpr int VD = DB / 4;
   u32x4 kw[HF], vw[VD];
   float ks, vs;
-  int nk;   // keys of the lane's unit that the cache holds
+  bool there;   // the lane's unit lies in a page of the cache
+  int32_t ek = kv8_entry(a, row, (key0 >> 4) + (c >> 2), key1), ev = kv8_entry(a, row, (key0 >> 4) + g, key1);
   const auto fetch = [&](int base) {
     const int uk = (base >> 4) + (c >> 2), uv = (base >> 4) + g;
-    bool okk, okv;
-    const int64_t pk = kv8_page(a, row, uk, uk * 16 < key1, &okk);
-    const int64_t pv = kv8_page(a, row, uv, uv * 16 < key1, &okv);
+    bool okk;
+    const int64_t pk = kv8_page(a, ek, &okk), pv = kv8_page(a, ev, &there);
     const int8_t* kp = a.k + (pk * a.kv_heads + h) * a.head_bytes + (uk & (a.units - 1)) * (16 * D) +
                        (4 * wave + (c & 3)) * D + g * 16;
     const int8_t* vp = a.v + (pv * a.kv_heads + h) * a.head_bytes + (uv & (a.units - 1)) * (16 * D) +
@@ -402,7 +418,8 @@ kv8_block_kernel(Kv8Args a) {
     const int64_t cell = (pv * a.kv_heads + h) * a.units + (uv & (a.units - 1));
     ks = a.ks[cell];
     vs = a.vs[cell];
-    nk = okv ? uv * 16 + 16 : 0;   // with the row's own limit below
+    ek = kv8_entry(a, row, uk + kKv8Tile / 16, key1);
+    ev = kv8_entry(a, row, uv + kKv8Tile / 16, key1);
   };
   const auto stage = [&](int buf) {
 #pragma unroll
@@ -422,35 +439,46 @@ kv8_block_kernel(Kv8Args a) {
     stage(0);
     int buf = 0;
     for (int base = key0; base < key1; base += kKv8Tile) {
-      const float ksc = ks, vsc = vs;
       const int ub = base + 16 * g;
-      const bool there = nk > 0;
+      const bool live = there && ub < key1;
+      const float ksc = live ? ks : 0.0f;   // whatever the scales of a unit that is not there are
+      const ValueScale vsc(live ? vs : 1.0f);
+      const int limit = live ? 16 : 0;
       __syncthreads();   // the tile is staged; nobody reads the other buffer any more
       const bool more = base + kKv8Tile < key1;
       if (more) fetch(base + kKv8Tile);
+      v4f s[2][4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) s[x][m] = v4f{qr[x].bias, qr[x].bias, qr[x].bias, qr[x].bias};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {   // an operand is read once for both row blocks
+          const v4i kk = kl[(buf * KO + m * KS + i) * kWave + lane];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) s[x][m] = mfma16<Fp16>(kk, qr[x].op[i], s[x][m]);
+        }
+      }
+      v4i p[2][2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        v4f s[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          s[m] = v4f{qr[x].bias, qr[x].bias, qr[x].bias, qr[x].bias};
-#pragma unroll
-          for (int i = 0; i < KS; ++i) s[m] = mfma16<Fp16>(kl[(buf * KO + m * KS + i) * kWave + lane], qr[x].op[i], s[m]);
-        }
-        const int nv = there ? min(max(seen[x] - ub, 0), 16) : 0;
-        v4i p[2];
+        const int nv = min(max(seen[x] - ub, 0), limit);
         const float before = sm[x].M;
-        const float alpha = softmax_tile(s, nv, qr[x].factor * (nv > 0 ? ksc : 0.0f), nv > 0 ? vsc : 1.0f, sm[x], p);
+        const float alpha = softmax_tile(s[x], nv, qr[x].factor * ksc, vsc, sm[x], p[x]);
         if (__any(sm[x].M != before)) {
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int v = 0; v < 4; ++v) o[x][d][v] *= alpha;
         }
+      }
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          o[x][d] = mfma16<Fp16>(vl[(buf * VO + 2 * d) * kWave + lane], p[0], o[x][d]);
-          o[x][d] = mfma16<Fp16>(vl[(buf * VO + 2 * d + 1) * kWave + lane], p[1], o[x][d]);
+      for (int d = 0; d < DB; ++d) {
+        const v4i v0 = vl[(buf * VO + 2 * d) * kWave + lane], v1 = vl[(buf * VO + 2 * d + 1) * kWave + lane];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          o[x][d] = mfma16<Fp16>(v0, p[x][0], o[x][d]);
+          o[x][d] = mfma16<Fp16>(v1, p[x][1], o[x][d]);
         }
       }
       buf ^= 1;
