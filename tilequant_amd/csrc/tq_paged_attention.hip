@@ -113,8 +113,10 @@ __device__ inline v4i widen_v(uint32_t lo, uint32_t hi) {
   return r;
 }
 
-__device__ inline uint32_t pack_h2(float a, float b) {
-  return (uint32_t)Fp16::from_f32(a) | ((uint32_t)Fp16::from_f32(b) << 16);
+__device__ inline uint32_t pack_h2(float a, float b) {   // round to nearest even
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
 }
 
 // One query row as B operands: lane (column c, group g) holds dimensions 64 hf + 16 g .. + 15 of its row (operand 2 hf:
@@ -183,23 +185,24 @@ struct ValueScale {
 };
 
 // The tile's probabilities as the P operands, from the raw products; returns the factor of what was summed before.
-// nv: how many of the lane's 16 keys its row sees (the lane's key index is 4 m + v).
-__device__ inline float softmax_tile(v4f (&s)[4], int nv, float f, const ValueScale& vs, Softmax& sm, v4i (&p)[2]) {
-  const float lv = vs.log;
-  const bool whole = __all(nv == 16);
-  if (!whole) {
+// live: the lane's unit counts; MASK: of its 16 keys (the lane's key index is 4 m + v) the row sees the first nv.
+template <bool MASK>
+__device__ __forceinline__ float softmax_tile(v4f (&s)[4], bool live, int nv, float f, const ValueScale& vs, Softmax& sm,
+                                              v4i (&p)[2]) {
+  if constexpr (MASK) {
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int v = 0; v < 4; ++v) s[m][v] = 4 * m + v < nv ? s[m][v] : -3.0e38f;
+    live = live && nv > 0;
   }
   float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
   for (int m = 1; m < 4; ++m) top = fmaxf(top, fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3])));
-  const float mine = nv > 0 ? fmaf(top, f, lv) : -INFINITY;
+  const float mine = live ? fmaf(top, f, vs.log) : -INFINITY;
   const float M = fmaxf(sm.M, g4_max(mine));
   const float ref = M == -INFINITY ? 0.0f : M;
-  const float c = lv - ref;
+  const float c = live ? vs.log - ref : -INFINITY;   // f is 0 where the unit does not count: the exponentials are 0
   float sum = 0.0f;
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
@@ -207,7 +210,7 @@ __device__ inline float softmax_tile(v4f (&s)[4], int nv, float f, const ValueSc
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       e[v] = __builtin_amdgcn_exp2f(fmaf(s[m][v], f, c));
-      if (!whole) e[v] = 4 * m + v < nv ? e[v] : 0.0f;
+      if constexpr (MASK) e[v] = 4 * m + v < nv ? e[v] : 0.0f;
       sum += e[v];
     }
     p[m >> 1][2 * (m & 1)] = (int)pack_h2(e[0], e[1]);
@@ -245,7 +248,7 @@ kv8_split_kernel(Kv8Args a) {
   const int r = r0 + c;
   const bool live = r < rows;
   const int qi = live ? r / a.G : 0, qh = live ? h * a.G + (r - qi * a.G) : 0;
-  const int seen = live ? sq.before + qi + 1 : 0;   // keys this lane's row sees
+  const int seen = live ? sq.before + qi + 1 : key1;   // keys this lane's row sees (rows past the last: any)
 
   QueryRow<XT, D> qr;
   qr.load(a.q + (int64_t)(sq.first + qi) * a.q_st + (int64_t)qh * a.q_sh, live, a, g);
@@ -279,6 +282,7 @@ kv8_split_kernel(Kv8Args a) {
     ev = kv8_entry(a, row, uv + NW * (kKv8Tile / 16), key1);
     const int nv = okv ? min(max(min(seen, key1) - uv * 16, 0), 16) : 0;
     if (nv == 0) ks = 0.0f, vs = 1.0f;   // whatever the scales of a page that is not there are
+    const bool whole = __all(nv == 16 || nv == 0);
 
     v4f s[4];
 #pragma unroll
@@ -292,7 +296,9 @@ kv8_split_kernel(Kv8Args a) {
     }
     v4i p[2];
     const float before = sm.M;
-    const float alpha = softmax_tile(s, nv, qr.factor * ks, ValueScale(vs), sm, p);
+    const ValueScale vsc(vs);
+    const float alpha = whole ? softmax_tile<false>(s, nv > 0, nv, qr.factor * ks, vsc, sm, p)
+                              : softmax_tile<true>(s, nv > 0, nv, qr.factor * ks, vsc, sm, p);
     if (__any(sm.M != before)) {
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -384,7 +390,7 @@ kv8_block_kernel(Kv8Args a) {
     const int r = r0 + wave * 32 + 16 * x + c;
     const bool live = r < rows;
     const int qi = live ? r / a.G : 0, qh = live ? h * a.G + (r - qi * a.G) : 0;
-    seen[x] = live ? min(sq.before + qi + 1, key1) : 0;
+    seen[x] = live ? min(sq.before + qi + 1, key1) : key1;   // rows past the last: any
     qr[x].load(a.q + (int64_t)(sq.first + qi) * a.q_st + (int64_t)qh * a.q_sh, live, a, g);
   }
   const int32_t* row = a.table + (int64_t)b * a.ld;
@@ -438,12 +444,13 @@ kv8_block_kernel(Kv8Args a) {
     fetch(key0);
     stage(0);
     int buf = 0;
+    // keys that every row of this wave sees
+    const int all = min(key1, sq.before + min((r0 + wave * 32) / a.G, sq.n - 1) + 1);
     for (int base = key0; base < key1; base += kKv8Tile) {
       const int ub = base + 16 * g;
       const bool live = there && ub < key1;
       const float ksc = live ? ks : 0.0f;   // whatever the scales of a unit that is not there are
       const ValueScale vsc(live ? vs : 1.0f);
-      const int limit = live ? 16 : 0;
       __syncthreads();   // the tile is staged; nobody reads the other buffer any more
       const bool more = base + kKv8Tile < key1;
       if (more) fetch(base + kKv8Tile);
@@ -460,17 +467,25 @@ kv8_block_kernel(Kv8Args a) {
         }
       }
       v4i p[2][2];
+      float alpha[2];
+      bool moved = false;
+      const bool whole = base + kKv8Tile <= all;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int nv = min(max(seen[x] - ub, 0), limit);
         const float before = sm[x].M;
-        const float alpha = softmax_tile(s[x], nv, qr[x].factor * ksc, vsc, sm[x], p[x]);
-        if (__any(sm[x].M != before)) {
+        if (whole)
+          alpha[x] = softmax_tile<false>(s[x], live, 16, qr[x].factor * ksc, vsc, sm[x], p[x]);
+        else
+          alpha[x] = softmax_tile<true>(s[x], live, min(max(seen[x] - ub, 0), 16), qr[x].factor * ksc, vsc, sm[x], p[x]);
+        moved |= sm[x].M != before;
+      }
+      if (__any(moved)) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) o[x][d][v] *= alpha;
-        }
+            for (int v = 0; v < 4; ++v) o[x][d][v] *= alpha[x];
       }
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
