@@ -352,7 +352,7 @@ kv8_split_kernel(Kv8Args a) {
 
 // ---- many query rows: tiles of 128 rows ---------------------------------------------
 //
-// Workgroup (row tile, sequence x kv head, split): four waves of 32 query rows each over 64-key tiles.  The four waves
+// Workgroup (sequence x kv head, row tile, split): four waves of 32 query rows each over 64-key tiles.  The four waves
 // widen a tile's codes once, a quarter each, into LDS in operand order (1 KiB per operand, lane after lane: no bank
 // conflicts either way), two tiles deep, and every wave multiplies its rows with all of them.
 constexpr int kKv8Block = 128;   // rows per workgroup
@@ -369,13 +369,14 @@ kv8_block_kernel(Kv8Args a) {
   v4i* vl = kl + 2 * KO * kWave;                        // [2][VO][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int b = blockIdx.y / a.kv_heads, h = blockIdx.y - b * a.kv_heads;
+  const int b = blockIdx.x / a.kv_heads, h = blockIdx.x - b * a.kv_heads;
   const int split = blockIdx.z;
   const Kv8Seq sq = kv8_seq(a, b);
   const int rows = sq.n * a.G;
-  // the last row tiles have the most keys: they go first
+  // The last row tiles have the most keys: they go first, over all sequences and heads (4 prompts of up to 2048
+  // tokens, 8 kv heads: 143 us, 173 with all tiles of a head before the next head's).
   const int tiles = (rows + kKv8Block - 1) / kKv8Block;
-  const int tile = tiles - 1 - (int)blockIdx.x;
+  const int tile = tiles - 1 - (int)blockIdx.y;
   if (tile < 0) return;
   const int r0 = tile * kKv8Block;
   const int last_i = min(sq.n - 1, (r0 + kKv8Block - 1) / a.G);
@@ -598,8 +599,20 @@ kv8_merge_kernel(Kv8Args a) {
 // ---- host ----------------------------------------------------------------------
 struct Kv8Plan {
   bool block;       // the 128-row kernel
+  int waves;        // of a split workgroup
   int row_tiles, n_splits, chunk;
 };
+
+// Split kernel: a workgroup's waves take 64 keys each in turn.  Up to kKv8Alone keys one workgroup of 8 waves takes a
+// sequence's kv head whole, which needs no join (one sequence of 613 tokens, 8 kv heads: 8.3 us, against 6.2 + 2.7 us and
+// a launch more in splits of 256).  Else 4 waves: one tile a wave while that makes at most kKv8Fine workgroups (32 ragged
+// sequences of up to 4099 tokens, 4 kv heads: 13.6 us, in chunks of 768 keys 16.4: the longest one's chain of tiles is
+// what is waited for); beyond, chunks that make kKv8Resident workgroups, three a compute unit, so that all run at once
+// (4 x 131072 tokens, 8 kv heads, in 4096 workgroups 200 us, in 1024 187, in 768 188).
+// 128-row kernel: split only where the row tiles do not fill the chip, in chunks of 512 keys or more.
+constexpr int kKv8Alone = 1024;
+constexpr int kKv8Resident = 768;
+constexpr int kKv8Fine = 3 * kKv8Resident;
 
 static Kv8Plan kv8_plan(int batch, int q_heads, int kv_heads, int max_query, int max_len) {
   Kv8Plan p;
@@ -608,15 +621,23 @@ static Kv8Plan kv8_plan(int batch, int q_heads, int kv_heads, int max_query, int
   const int per = p.block ? kKv8Block : kKv8Rows;
   p.row_tiles = (int)((rows + per - 1) / per);
   const int64_t groups = (int64_t)batch * kv_heads * p.row_tiles;
-  const int64_t want = p.block ? 512 : 1024;       // workgroups
-  const int64_t step = p.block ? 512 : 256;        // the shortest split, in keys
-  const int64_t most = (max_len + step - 1) / step;
-  int64_t splits = want / groups;
-  splits = splits < 1 ? 1 : splits > most ? most : splits;
-  if (splits < 1) splits = 1;
-  int64_t chunk = (max_len + splits - 1) / splits;
-  chunk = (chunk + step - 1) / step * step;
-  if (chunk < step) chunk = step;
+  p.waves = 4;
+  int64_t chunk;
+  if (p.block) {
+    const int64_t most = (max_len + 511) / 512;
+    int64_t splits = 512 / groups;
+    splits = splits < 1 ? 1 : splits > most ? most : splits;
+    chunk = splits > 1 ? ((max_len + splits - 1) / splits + kKv8Tile - 1) / kKv8Tile * kKv8Tile : max_len;
+  } else if (max_len <= kKv8Alone) {
+    p.waves = 8;
+    chunk = max_len;
+  } else {
+    const int64_t step = 4 * kKv8Tile;
+    const int64_t fine = groups * ((max_len + step - 1) / step);
+    chunk = fine <= kKv8Fine ? step : step * ((fine + kKv8Resident - 1) / kKv8Resident);
+  }
+  if (chunk < kKv8Tile) chunk = kKv8Tile;
+  if (chunk > (1 << 30)) chunk = 1 << 30;
   p.chunk = (int)chunk;
   p.n_splits = (int)((max_len + chunk - 1) / chunk);
   if (p.n_splits < 1) p.n_splits = 1;
@@ -628,11 +649,14 @@ static int kv8_launch(const Kv8Args& a, const Kv8Plan& p, hipStream_t s) {
   if (p.block) {
     constexpr size_t lds = (size_t)2 * (4 * (D / 32) + 2 * (D / 16)) * 1024;
     TQ_RETURN_IF_HIP_ERROR((allow_lds<kv8_block_kernel<XT, D>>(lds)));
-    hipLaunchKernelGGL((kv8_block_kernel<XT, D>), dim3(p.row_tiles, a.batch * a.kv_heads, p.n_splits),
+    hipLaunchKernelGGL((kv8_block_kernel<XT, D>), dim3(a.batch * a.kv_heads, p.row_tiles, p.n_splits),
                        dim3(kKv8Waves * kWave), lds, s, a);
   } else {
-    hipLaunchKernelGGL((kv8_split_kernel<XT, D, 4>), dim3(p.n_splits, a.batch * a.kv_heads, p.row_tiles), dim3(256), 0,
-                       s, a);
+    const dim3 grid(p.n_splits, a.batch * a.kv_heads, p.row_tiles);
+    if (p.waves == 8)
+      hipLaunchKernelGGL((kv8_split_kernel<XT, D, 8>), grid, dim3(8 * kWave), 0, s, a);
+    else
+      hipLaunchKernelGGL((kv8_split_kernel<XT, D, 4>), grid, dim3(4 * kWave), 0, s, a);
   }
   if (p.n_splits > 1)
     hipLaunchKernelGGL((kv8_merge_kernel<XT, D>), dim3((unsigned)(((int64_t)a.tokens * a.q_heads + 3) / 4)), dim3(256),
