@@ -18,7 +18,9 @@ namespace tq {
 //   Granted rows pop their pages in row order and get the next places of the slot list.
 // The sums are exclusive / inclusive prefix sums over the rows, so one workgroup does them (a chunk of one row per
 // thread at a time, carries in registers); pages and tokens are then dealt to the threads flat, each finding its row by
-// a binary search in the chunk's prefix sums in LDS.
+// a binary search in the chunk's prefix sums in LDS.  What it moves is little (8 bytes a token); the bound is the chain
+// of waits of one workgroup: 64 rows with a token each 4 us, about an empty launch; 256 rows that all end and take 115
+// thousand tokens (12 thousand pages, every page's and token's row searched for) 19 us with the slots' launch.
 constexpr int kTabThreads = 1024;
 
 struct TablesArgs {
@@ -64,15 +66,17 @@ __device__ inline Pair64 scan_inclusive(Pair64 x, Pair64* wave_sums) {
   return x;
 }
 
-// Last index i in [0, n) with start[i] <= x (start ascending, start[0] <= x).
-__device__ inline int last_at_most(const int64_t* start, int n, int64_t x) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] <= x) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+// Per item: the last index r in [0, N) with start[r] <= x (start ascending, start[0] <= x; N a power of two).  The
+// items' searches run side by side: one alone waits for LDS log2(N) times.
+constexpr int kFlat = 4;
+template <int N>
+__device__ __forceinline__ void last_at_most(const int64_t* start, const int64_t (&x)[kFlat], int (&r)[kFlat]) {
+#pragma unroll
+  for (int j = 0; j < kFlat; ++j) r[j] = 0;
+#pragma unroll
+  for (int step = N / 2; step > 0; step >>= 1)
+#pragma unroll
+    for (int j = 0; j < kFlat; ++j) r[j] = start[r[j] + step] <= x[j] ? r[j] + step : r[j];
 }
 
 // A page that is not one of the cache's (a damaged list) gives a slot that the cache's kernels skip, or another page's.
@@ -95,18 +99,30 @@ tables_step_kernel(TablesArgs a) {
       const int b = r0 + t;
       int held = 0;
       if (b < a.rows && a.finished[b])
-        held = min((int)(((int64_t)max(a.lengths[b], 0) + a.block - 1) / a.block), a.width);
+        held = min((int)(((uint32_t)max(a.lengths[b], 0) + a.block - 1) / (uint32_t)a.block), a.width);
       const Pair64 inc = scan_inclusive<NT>(Pair64{held, 0}, wave_sums);
       start_pages[t] = inc.a - held;
       if (t == NT - 1) total = inc;
       __syncthreads();
       const int64_t n = total.a;
-      for (int64_t i = t; i < n; i += NT) {
-        const int r = last_at_most(start_pages, NT, i);
-        int32_t* entry = a.table + (int64_t)(r0 + r) * a.ld + (i - start_pages[r]);
-        const int64_t at = count0 + pushed + i;
-        if (at < a.free_cap) a.free_list[at] = *entry;
-        *entry = -1;
+      for (int64_t i0 = t; i0 < n; i0 += kFlat * NT) {
+        int64_t i[kFlat];
+        int r[kFlat], page[kFlat];
+        int32_t* entry[kFlat];
+#pragma unroll
+        for (int j = 0; j < kFlat; ++j) i[j] = i0 + j * NT;
+        last_at_most<NT>(start_pages, i, r);
+#pragma unroll
+        for (int j = 0; j < kFlat; ++j) {
+          entry[j] = a.table + (int64_t)(r0 + r[j]) * a.ld + (i[j] - start_pages[r[j]]);
+          if (i[j] < n) page[j] = *entry[j];
+        }
+#pragma unroll
+        for (int j = 0; j < kFlat; ++j) {
+          const int64_t at = count0 + pushed + i[j];
+          if (i[j] < n && at < a.free_cap) a.free_list[at] = page[j];
+          if (i[j] < n) *entry[j] = -1;
+        }
       }
       pushed += n;
       __syncthreads();   // the next chunk writes the sums; the pops below read the list
@@ -125,8 +141,9 @@ tables_step_kernel(TablesArgs a) {
       len = (a.finished != nullptr && a.finished[b]) ? 0 : max(a.lengths[b], 0);
       n = max(a.new_tokens[b], 0);
       fits = len + n <= (int64_t)a.width * a.block;
-      have = (len + a.block - 1) / a.block;
-      need = fits ? (len + n + a.block - 1) / a.block - have : 0;
+      // 32 bits hold these: len < 2^31, and len + n <= width * block < 2^31 where it fits
+      have = ((uint32_t)len + a.block - 1) / (uint32_t)a.block;
+      need = fits ? ((uint32_t)(len + n) + a.block - 1) / (uint32_t)a.block - have : 0;
     }
     const Pair64 inc = scan_inclusive<NT>(Pair64{need, fits ? n : 0}, wave_sums);
     const bool ok = live && fits && (need == 0 || asked.a + inc.a <= count) && asked.b + inc.b <= a.max_tokens;
@@ -147,20 +164,42 @@ tables_step_kernel(TablesArgs a) {
     }
     __syncthreads();
     const Pair64 chunk = total;
-    for (int64_t i = t; i < chunk.a; i += NT) {
-      const int r = last_at_most(start_pages, NT, i);
-      a.table[(int64_t)(r0 + r) * a.ld + row_have[r] + (i - start_pages[r])] = a.free_list[count - 1 - taken.a - i];
+    for (int64_t i0 = t; i0 < chunk.a; i0 += kFlat * NT) {
+      int64_t i[kFlat];
+      int r[kFlat], page[kFlat];
+#pragma unroll
+      for (int j = 0; j < kFlat; ++j) {
+        i[j] = i0 + j * NT;
+        if (i[j] < chunk.a) page[j] = a.free_list[count - 1 - taken.a - i[j]];
+      }
+      last_at_most<NT>(start_pages, i, r);
+#pragma unroll
+      for (int j = 0; j < kFlat; ++j)
+        if (i[j] < chunk.a) a.table[(int64_t)(r0 + r[j]) * a.ld + row_have[r[j]] + (i[j] - start_pages[r[j]])] = page[j];
     }
     if constexpr (TOKENS) {
-      for (int64_t i = t; i < chunk.b; i += NT) {
-        const int r = last_at_most(start_tokens, NT, i);
-        const int64_t pos = row_len[r] + (i - start_tokens[r]);
-        const int page_at = (int)(pos / a.block);
-        const int32_t page = page_at < row_have[r]
-                                 ? a.table[(int64_t)(r0 + r) * a.ld + page_at]
-                                 : a.free_list[count - 1 - taken.a - (start_pages[r] + page_at - row_have[r])];
-        a.slots[taken.b + i] = page < 0 ? -1 : slot_of(page, a.block, (int)(pos - (int64_t)page_at * a.block));
-        a.positions[taken.b + i] = (int32_t)pos;
+      for (int64_t i0 = t; i0 < chunk.b; i0 += kFlat * NT) {
+        int64_t i[kFlat];
+        int r[kFlat], page[kFlat];
+        uint32_t pos[kFlat], page_at[kFlat];
+#pragma unroll
+        for (int j = 0; j < kFlat; ++j) i[j] = i0 + j * NT;
+        last_at_most<NT>(start_tokens, i, r);
+#pragma unroll
+        for (int j = 0; j < kFlat; ++j) {
+          pos[j] = (uint32_t)(row_len[r[j]] + (i[j] - start_tokens[r[j]]));
+          page_at[j] = pos[j] / (uint32_t)a.block;
+          const int64_t fresh = (int64_t)page_at[j] - row_have[r[j]];   // < 0: a page that the row had
+          const int32_t* from = fresh < 0 ? a.table + (int64_t)(r0 + r[j]) * a.ld + page_at[j]
+                                          : a.free_list + (count - 1 - taken.a - (start_pages[r[j]] + fresh));
+          if (i[j] < chunk.b) page[j] = *from;
+        }
+#pragma unroll
+        for (int j = 0; j < kFlat; ++j) {
+          if (i[j] >= chunk.b) continue;
+          a.slots[taken.b + i[j]] = page[j] < 0 ? -1 : slot_of(page[j], a.block, (int)(pos[j] - page_at[j] * a.block));
+          a.positions[taken.b + i[j]] = (int32_t)pos[j];
+        }
       }
     }
     asked.a += carry.a;
@@ -209,31 +248,68 @@ tables_slots_kernel(TablesArgs a) {
 // Per unit and head, over the new tokens x of the unit (a: their absmax; below 2^-100 it counts as 0):
 //   s = max(s_old, a / 127),  s_old = 0 when no older token is in the unit;  new codes rint(x (1 / s));
 //   older codes c become rint(c (s_old / s)) when the scale grew.  All fp32, divisions correctly rounded.
-// One wave per (token, head, K or V); the wave of a unit's first new token takes the whole unit, the others end at once
-// (they cost less than a list of units would).  The bound is memory: 16-bit rows in, codes out.
+// One wave takes the units whose first new token is among its `window` tokens of the list, for one head of K or V; it
+// sees which those are from the slots themselves, so no list of units is made.  A window of 16 tokens holds the start
+// of about one unit of a prompt; a window of 1 keeps a decoding step's units, one token each, on a wave each.
+// The bound is memory: 16-bit rows in, codes out.  4 prompts of 2048 tokens, 8 kv heads of 128: 50 MB in 14.5 us,
+// 3.5 TB/s where a large copy reaches 4.9 (one wave a token, clamps and roundings in fp32, loads behind branches: 38).
 struct AppendArgs {
   const uint16_t* x[2];
   int64_t x_st[2], x_sh[2];
   const int32_t* slots;
   int8_t* codes[2];
   float* scales[2];
-  int tokens, kv_heads, units;   // units per page
+  int tokens, window, kv_heads, units;   // units per page
   int unit_shift;                // log2(units)
   int64_t n_slots;
 };
 
 constexpr float kTinyAbsmax = 7.888609052210118e-31f;   // 2^-100
 
+// Two 16-bit values in a word, as bits: |x| orders like the integers.
+template <class XT>
+constexpr uint32_t kInfBits = std::is_same<XT, Bf16>::value ? 0x7f80u : 0x7c00u;
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t w) {   // both halves
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
 // NaN -> 0, infinities -> the largest finite value
 template <class XT>
-__device__ inline float finite(float x) {
-  constexpr float top = std::is_same<XT, Bf16>::value ? 3.3895313892515355e38f : 65504.0f;
-  return x != x ? 0.0f : fminf(fmaxf(x, -top), top);
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int sh = 0; sh < 32; sh += 16) {
+    const uint32_t x = (w >> sh) & 0xffffu, m = x & 0x7fffu;
+    r |= (m < kInfBits<XT> ? x : m == kInfBits<XT> ? x - 1 : 0u) << sh;
+  }
+  return r;
 }
 
-__device__ inline uint32_t code_byte(float v) {   // rint and clamp to a signed byte
-  return (uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_rintf(v), -127.0f, 127.0f) & 0xffu;
+// The absmax of the unit whose values the wave's lanes hold; values that are not finite are replaced in place.
+template <class XT, int N>
+__device__ __forceinline__ float unit_absmax(uint32_t (&v)[N]) {
+  for (;;) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max_abs2(m, v[i]);
+    m = max(m & 0xffffu, m >> 16);
+    m = __float_as_uint(wave_max_nonneg(__uint_as_float(m)));   // an integer maximum over the lanes
+    if (m < kInfBits<XT>) return XT::to_f32((uint16_t)m);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = finite2<XT>(v[i]);
+  }
 }
+
+// rint(x r) in the low byte: |x r| <= 127 (1 + 2^-22), and adding 1.5 * 2^23 rounds to an integer, ties to even
+__device__ __forceinline__ uint32_t code_of(float x, float r) { return __float_as_uint(x * r + 12582912.0f); }
+__device__ __forceinline__ uint32_t bytes4(uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {   // the low bytes
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b3, b2, 0x0c0c0400u), __builtin_amdgcn_perm(b1, b0, 0x0c0c0400u),
+                               0x05040100u);
+}
+template <class XT>
+__device__ __forceinline__ float half_of(uint32_t w, int i) { return XT::to_f32((uint16_t)(w >> (16 * i))); }
 __device__ inline float byte_code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
 struct UnitScale {
@@ -248,127 +324,162 @@ struct UnitScale {
   }
 };
 
+// One unit of one head: `src` names each offset's new token (-1: none), `first` is one of them.
 template <class XT, int D>
-__global__ void __launch_bounds__(256)
-kv8_append_kernel(AppendArgs a) {
-  __shared__ int src_all[4][16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x * 4 + wave;
-  const int h = blockIdx.y, kv = blockIdx.z;
-  if (t >= a.tokens) return;
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.n_slots) return;
-  const int64_t unit = slot >> 4;   // over all pages
-  if (t > 0) {
-    const int64_t prev = a.slots[t - 1];
-    if (prev >= 0 && (prev >> 4) == unit) return;   // not the unit's first new token
-  }
-  // the run of tokens of this unit: each offset's source is the last token that names it
-  int* src_of = src_all[wave];
-  if (lane < 16) src_of[lane] = -1;
-  __builtin_amdgcn_wave_barrier();
-  for (int t0 = t; t0 < a.tokens; t0 += kWave) {
-    const int tt = t0 + lane;
-    const int64_t sl = tt < a.tokens ? (int64_t)a.slots[tt] : -1;
-    const uint64_t in = __ballot(sl >= 0 && (sl >> 4) == unit);
-    const int n = in == ~0ull ? kWave : __builtin_ctzll(~in);
-    if (lane < n) atomicMax(&src_of[sl & 15], tt);
-    if (n < kWave) break;
-  }
-  __builtin_amdgcn_s_waitcnt(0xC07F);   // LDS operations of this wave
-  asm volatile("" ::: "memory");
-  int src[16];
+__device__ __forceinline__ void append_unit(const AppendArgs& a, int h, int kv, int64_t unit, const int (&src)[16],
+                                            int first) {
+  const int lane = threadIdx.x & 63;
   int begun = 16;   // the unit held tokens 0 .. begun - 1 before
+  bool whole = true;
 #pragma unroll
   for (int o = 15; o >= 0; --o) {
-    src[o] = __builtin_amdgcn_readfirstlane(src_of[o]);
     if (src[o] >= 0) begun = o;
+    else whole = false;
   }
-  const int64_t page = unit >> a.unit_shift;
-  const int64_t cell = (page * a.kv_heads + h) * a.units + (unit & (a.units - 1));   // (page, head, unit)
+  const int64_t cell = ((unit >> a.unit_shift) * a.kv_heads + h) * a.units + (unit & (a.units - 1));
   float* scale_at = a.scales[kv] + cell;
   int8_t* codes = a.codes[kv] + cell * (16 * D);
   const float old = begun > 0 ? *scale_at : 0.0f;
   const uint16_t* x = a.x[kv] + (int64_t)h * a.x_sh[kv];
 
+  // All loads are issued before the first is used: an offset without a new token reads `first` and drops it.
   if (kv == 0) {
     // lane: 8 dimensions of every kRows-th token
     constexpr int kLanes = D / 8, kRows = kWave / kLanes, kSteps = 16 / kRows;
     const int ch = lane % kLanes, rg = lane / kLanes;
-    u32x4 v[kSteps];
+    uint32_t v[kSteps * 4];
     u32x2 oc[kSteps];
     int sr[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      const int o = rg + kRows * i;
-      sr[i] = src_of[o];
-      v[i] = u32x4{0, 0, 0, 0};
-      oc[i] = u32x2{0, 0};
-      if (sr[i] >= 0) v[i] = *reinterpret_cast<const u32x4*>(x + (int64_t)sr[i] * a.x_st[0] + ch * 8);
-      else if (o < begun) oc[i] = *reinterpret_cast<const u32x2*>(codes + o * D + ch * 8);
+      sr[i] = src[kRows * i];
+#pragma unroll
+      for (int r = 1; r < kRows; ++r) sr[i] = rg == r ? src[kRows * i + r] : sr[i];
+      const int row = sr[i] >= 0 ? sr[i] : first;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(x + (int64_t)row * a.x_st[0] + ch * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = w[e];
     }
-    float f[kSteps][8], m = 0.0f;
+    if (begun > 0) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) oc[i] = *reinterpret_cast<const u32x2*>(codes + (rg + kRows * i) * D + ch * 8);
+    }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[i][e] = finite<XT>(XT::to_f32((uint16_t)(v[i][e >> 1] >> (16 * (e & 1)))));
-        m = fmaxf(m, fabsf(f[i][e]));
-      }
-    const UnitScale u(wave_max_nonneg(m), old);
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = sr[i] >= 0 ? v[4 * i + e] : 0u;
+    const UnitScale u(unit_absmax<XT>(v), old);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      const int o = rg + kRows * i;
-      u32x2 w{0, 0};
+      u32x2 w;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        w[e >> 2] |= code_byte(sr[i] >= 0 ? f[i][e] * u.inv : byte_code(oc[i][e >> 2], e & 3) * u.shrink) << (8 * (e & 3));
-      if (sr[i] >= 0 || (o < begun && u.grew)) *reinterpret_cast<u32x2*>(codes + o * D + ch * 8) = w;
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t lo = v[4 * i + 2 * p], hi = v[4 * i + 2 * p + 1];
+        w[p] = bytes4(code_of(half_of<XT>(lo, 0), u.inv), code_of(half_of<XT>(lo, 1), u.inv),
+                      code_of(half_of<XT>(hi, 0), u.inv), code_of(half_of<XT>(hi, 1), u.inv));
+      }
+      if (sr[i] >= 0) *reinterpret_cast<u32x2*>(codes + (rg + kRows * i) * D + ch * 8) = w;
+    }
+    if (begun > 0 && u.grew) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        u32x2 w;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          w[p] = bytes4(code_of(byte_code(oc[i][p], 0), u.shrink), code_of(byte_code(oc[i][p], 1), u.shrink),
+                        code_of(byte_code(oc[i][p], 2), u.shrink), code_of(byte_code(oc[i][p], 3), u.shrink));
+        if (rg + kRows * i < begun) *reinterpret_cast<u32x2*>(codes + (rg + kRows * i) * D + ch * 8) = w;
+      }
     }
     if (lane == 0) *scale_at = u.s;
   } else {
     // lane: all 16 tokens of kDims dimensions (a unit's row of 16 bytes each)
     constexpr int kDims = D / kWave;
+    uint32_t v[16];
     u32x4 oc[kDims];
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) {
-      oc[d] = u32x4{0, 0, 0, 0};
-      if (begun > 0 || src[15] < 0) oc[d] = *reinterpret_cast<const u32x4*>(codes + (lane * kDims + d) * 16);
-    }
-    uint32_t v[16];
-#pragma unroll
     for (int o = 0; o < 16; ++o) {
-      v[o] = 0;
-      if (src[o] >= 0) {
-        const uint16_t* p = x + (int64_t)src[o] * a.x_st[1] + lane * kDims;
-        if constexpr (kDims == 2) v[o] = *reinterpret_cast<const uint32_t*>(p);
-        else v[o] = *p;
-      }
+      const uint16_t* p = x + (int64_t)(src[o] >= 0 ? src[o] : first) * a.x_st[1] + lane * kDims;
+      if constexpr (kDims == 2) v[o] = *reinterpret_cast<const uint32_t*>(p);
+      else v[o] = *p;
     }
-    float f[16][kDims], m = 0.0f;
+    if (!whole) {
 #pragma unroll
-    for (int o = 0; o < 16; ++o)
+      for (int d = 0; d < kDims; ++d) oc[d] = *reinterpret_cast<const u32x4*>(codes + (lane * kDims + d) * 16);
+    }
 #pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        f[o][d] = finite<XT>(XT::to_f32((uint16_t)(v[o] >> (16 * d))));
-        m = fmaxf(m, fabsf(f[o][d]));
-      }
-    const UnitScale u(wave_max_nonneg(m), old);
+    for (int o = 0; o < 16; ++o) v[o] = src[o] >= 0 ? v[o] : 0u;
+    const UnitScale u(unit_absmax<XT>(v), old);
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
-      u32x4 w = oc[d];
+      u32x4 w;
 #pragma unroll
-      for (int o = 0; o < 16; ++o) {
-        const int sh = 8 * (o & 3);
-        const bool now = src[o] >= 0;
-        if (now || (o < begun && u.grew)) {
-          const uint32_t c = code_byte(now ? f[o][d] * u.inv : byte_code(oc[d][o >> 2], o & 3) * u.shrink);
-          w[o >> 2] = (w[o >> 2] & ~(0xffu << sh)) | (c << sh);
+      for (int p = 0; p < 4; ++p)
+        w[p] = bytes4(code_of(half_of<XT>(v[4 * p], d), u.inv), code_of(half_of<XT>(v[4 * p + 1], d), u.inv),
+                      code_of(half_of<XT>(v[4 * p + 2], d), u.inv), code_of(half_of<XT>(v[4 * p + 3], d), u.inv));
+      if (!whole) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          uint32_t now = 0, c = oc[d][p];
+          if (begun > 0 && u.grew)
+            c = bytes4(code_of(byte_code(c, 0), u.shrink), code_of(byte_code(c, 1), u.shrink),
+                       code_of(byte_code(c, 2), u.shrink), code_of(byte_code(c, 3), u.shrink));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) now |= src[4 * p + e] >= 0 ? 0xffu << (8 * e) : 0u;
+          uint32_t kept = 0;   // offsets at and above `begun` without a new token stay as they were
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kept |= 4 * p + e >= begun ? 0xffu << (8 * e) : 0u;
+          w[p] = (w[p] & now) | (((c & ~kept) | (oc[d][p] & kept)) & ~now);
         }
       }
       *reinterpret_cast<u32x4*>(codes + (lane * kDims + d) * 16) = w;
     }
     if (lane == 0) *scale_at = u.s;
+  }
+}
+
+template <class XT, int D>
+__global__ void __launch_bounds__(256)
+kv8_append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * a.window;
+  const int h = blockIdx.y, kv = blockIdx.z;
+  if (t0 >= a.tokens) return;
+  // the unit of each lane's token (-1: none), and of the token before it
+  const auto load_slot = [&](int64_t t) {
+    const int32_t s = t < a.tokens ? a.slots[t] : -1;
+    return s < a.n_slots ? s : -1;
+  };
+  const int slot = load_slot(t0 + lane), unit = slot < 0 ? -1 : slot >> 4;
+  int before = __shfl_up(unit, 1);
+  if (lane == 0) before = t0 > 0 ? load_slot(t0 - 1) : -1, before = before < 0 ? -1 : before >> 4;
+  uint32_t todo = (uint32_t)__ballot(lane < a.window && unit >= 0 && unit != before);   // window <= 16
+  for (; todo; todo &= todo - 1) {
+    const int i = __builtin_ctz(todo);
+    const int mine = __builtin_amdgcn_readlane(unit, i);
+    // the run of tokens of this unit; each offset's source is the last token that names it
+    int src[16];
+#pragma unroll
+    for (int o = 0; o < 16; ++o) src[o] = -1;
+    int64_t base = t0;
+    int at = slot, at_unit = unit;
+    uint64_t skip = (1ull << i) - 1;   // lanes before the run
+    for (;;) {
+      const uint64_t out = ~(__ballot(at_unit == mine) | skip);
+      const uint64_t run = (out ? (out & (0 - out)) - 1 : ~0ull) & ~skip;
+#pragma unroll
+      for (int o = 0; o < 16; ++o) {
+        const uint64_t named = __ballot((at & 15) == o) & run;
+        if (named) src[o] = (int)(base + 63 - __builtin_clzll(named));
+      }
+      if (out) break;
+      base += kWave;
+      if (base >= a.tokens) break;
+      at = load_slot(base + lane);
+      at_unit = at < 0 ? -1 : at >> 4;
+      skip = 0;
+    }
+    append_unit<XT, D>(a, h, kv, mine, src, (int)t0 + i);
   }
 }
 
@@ -471,6 +582,21 @@ static int check_cache(const tq_kv8_cache* c) {
   return TQ_OK;
 }
 
+// Waves of window 1 end at once unless their token begins a unit, 15 of 16 in a prompt; wide windows make a wave of a
+// decoding step append unit after unit, 2 us each.  So: 2048 to 4096 waves, as far as a window of 16 goes.  Measured in
+// us at 8 kv heads of 128, windows 1 / 2 / 4 / 8 / 16:
+//   64 requests of one token     4.2   6.1  10.0  17.9  33.1   (rule: 1)
+//   512 requests of one token   11.7  11.2  12.8  18.8  34.2   (2)
+//   a prompt of 512              6.8   4.7   5.3   5.4   5.3   (2)
+//   512 requests of 4 tokens    27.8  20.9  20.3  20.6  24.1   (8)
+//   4 prompts of 2048           60.0  33.4  22.0  17.4  14.2   (16)
+static int append_window(int tokens, int kv_heads) {
+  const int64_t rows = (int64_t)tokens * kv_heads;
+  int window = 1;
+  while (window < 16 && rows > 2048 * (int64_t)window) window *= 2;
+  return window;
+}
+
 static int log2_exact(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 }  // namespace tq
@@ -517,12 +643,13 @@ extern "C" int tq_kv8_append(const tq_kv8_cache* cache, const void* k, int64_t k
     return TQ_ERR_ALIGN;
   if (cache->kv_heads > 65535) return TQ_ERR_ARG;
   const int units = cache->block / 16;
+  const int window = append_window(tokens, cache->kv_heads);
   const AppendArgs a{{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v)},
                      {k_stride_t, v_stride_t}, {k_stride_h, v_stride_h}, slots,
                      {cache->k_codes, cache->v_codes}, {cache->k_scales, cache->v_scales},
-                     tokens, cache->kv_heads, units, log2_exact(units), (int64_t)cache->pages * cache->block};
+                     tokens, window, cache->kv_heads, units, log2_exact(units), (int64_t)cache->pages * cache->block};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 g((tokens + 3) / 4, cache->kv_heads, 2);
+  const dim3 g((tokens + 4 * window - 1) / (4 * window), cache->kv_heads, 2);
   const bool bf = dtype == TQ_DTYPE_BF16;
   if (cache->head_dim == 128) {
     if (bf) hipLaunchKernelGGL((kv8_append_kernel<Bf16, 128>), g, dim3(256), 0, s, a);
