@@ -194,6 +194,34 @@ def test_append_one_slot_named_a_hundred_times():
     c.check()
 
 
+@pytest.mark.parametrize("dim,heads,tokens", [(128, 150, 15), (64, 150, 29), (128, 150, 60), (64, 150, 250), (128, 9, 3700)])
+def test_append_long_lists_of_mixed_runs(dim, heads, tokens):
+    """Runs of 1 to 70 slots from any offset, doubled slots, skipped entries: waves take several units, or none."""
+    block, pages = 16, tokens // 4 + 80
+    c = Cache(pages, heads, dim, block, seed=tokens)
+    g, slots, page = gen(tokens), [], 0
+    while len(slots) < tokens:
+        n, at = (int(torch.randint(1, 71, (), generator=g)) if torch.rand((), generator=g) < 0.4 else 1), \
+            int(torch.randint(0, 16, (), generator=g))
+        run_ = [page * block + at + i for i in range(n)]
+        page = run_[-1] // block + 1                 # a unit is in one run only
+        kind = int(torch.randint(0, 4, (), generator=g))
+        slots += run_ + ([run_[-1]] * 2 if kind == 0 else [-1] if kind == 1 else [])
+    slots = [x if x < pages * block else -1 for x in slots[:tokens]]
+    k, v = (rows_of((tokens, heads, dim), torch.bfloat16, tokens + i, spread=4.0) for i in range(2))
+    c.append(k.to(DEV), v.to(DEV), slots)
+    ref.append(finite(k), c.k, c.ks, slots, False)
+    ref.append(finite(v), c.v, c.vs, slots, True)
+    c.check()
+
+
+def test_the_tensors_stay_the_objects_own():
+    c, t = Cache(2, 1, 64, 16), TablesPair(2, 2, 4, 16)
+    for obj, name in ((c.gpu, "k_codes"), (c.gpu, "v_scales"), (t.gpu, "lengths"), (t.gpu, "block_table")):
+        with pytest.raises(AttributeError):
+            setattr(obj, name, getattr(obj, name).clone())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_append_not_finite_zero_and_tiny(dtype):
     c = Cache(2, 2, 128, 16, fill=False)

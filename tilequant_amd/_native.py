@@ -241,6 +241,19 @@ def stream_handle(device: torch.device) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
 
 
+def launch(device: torch.device, what: str, fn, *args) -> None:
+    """Call an entry point whose last argument is the stream, on the current stream of ``device`` with that device
+    current, and check its status.  The context manager that makes it current is entered only where it is not."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc:
+        check(rc, what)
+
+
 def capture_id(stream: int) -> Optional[int]:
     """The graph capture that ``stream`` is in: 0 for none, its id, or None when
     that cannot be told."""

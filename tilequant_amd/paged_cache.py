@@ -23,6 +23,7 @@ Every call only enqueues work on the current stream of the tensors' device.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -38,7 +39,7 @@ def _check_block(block_size: int) -> None:
 
 
 def _int32(name: str, t: torch.Tensor, shape, device) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
 
 
@@ -75,9 +76,15 @@ class BlockTables:
         _int32("free_count", free_count, (1,), block_table.device)
         if max(width, free_blocks.numel()) * block_size >= 1 << 31:
             raise ValueError("slots are 32-bit: pages * block size must stay below 2^31")
-        self.block_table, self.lengths = block_table, lengths
-        self.free_blocks, self.free_count = free_blocks, free_count
+        self._tensors = block_table, lengths, free_blocks, free_count   # held, as their addresses are below
         self.block_size = int(block_size)
+        self._state = (block_table.data_ptr(), max(block_table.stride(0), width), lengths.data_ptr(),
+                       free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr())
+
+    block_table = property(lambda self: self._tensors[0])
+    lengths = property(lambda self: self._tensors[1])
+    free_blocks = property(lambda self: self._tensors[2])
+    free_count = property(lambda self: self._tensors[3])
 
     @classmethod
     def allocate(cls, *, requests: int, blocks_per_request: int, blocks: int, block_size: int = 64,
@@ -108,22 +115,22 @@ class BlockTables:
         # one allocation for the three int32 results
         out = torch.empty((2 * max_tokens + rows + 1,), dtype=torch.int32, device=dev)
         granted = torch.empty((rows,), dtype=torch.bool, device=dev)
-        slots, positions, starts = out[:max_tokens], out[max_tokens:2 * max_tokens], out[2 * max_tokens:]
-        with torch.cuda.device(dev):
-            rc = nat.lib().tq_block_tables_step(
-                nat.ptr(new_tokens), nat.ptr(finished), nat.ptr(self.block_table), max(self.block_table.stride(0), width),
-                nat.ptr(self.lengths), nat.ptr(self.free_blocks), self.free_blocks.numel(), nat.ptr(self.free_count),
-                nat.ptr(slots), nat.ptr(positions), nat.ptr(starts), nat.ptr(granted), rows, width, self.block_size,
-                max_tokens, nat.stream_handle(dev))
-        nat.check(rc, "tq_block_tables_step")
-        return StepSlots(slots, positions, starts, granted)
+        at = out.data_ptr()
+        nat.launch(dev, "tq_block_tables_step", nat.lib().tq_block_tables_step,
+                   new_tokens.data_ptr(), nat.ptr(finished), *self._state, at, at + 4 * max_tokens, at + 8 * max_tokens,
+                   granted.data_ptr(), rows, width, self.block_size, max_tokens)
+        return StepSlots(out[:max_tokens], out[max_tokens:2 * max_tokens], out[2 * max_tokens:], granted)
+
+
+@lru_cache(maxsize=1024)
+def _attention_elems(*sizes: int) -> int:
+    return int(nat.lib().tq_kv8_attention_workspace_elems(*sizes))
 
 
 def paged_attention_workspace(tokens: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, max_query: int,
                               max_length: int, device) -> Optional[torch.Tensor]:
     """fp32 scratch for the split partials of ``PagedKVCache.attend``; None when the call needs none."""
-    elems = int(nat.lib().tq_kv8_attention_workspace_elems(tokens, batch, q_heads, kv_heads, head_dim, max_query,
-                                                           max_length))
+    elems = _attention_elems(tokens, batch, q_heads, kv_heads, head_dim, max_query, max_length)
     return torch.empty((elems,), device=device, dtype=torch.float32) if elems else None
 
 
@@ -154,13 +161,18 @@ class PagedKVCache:
         for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
             if tuple(t.shape) != (layers, pages, kv_heads, units):
                 raise ValueError(f"{name} must be [layers, pages, kv_heads, block / 16]")
-        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+        self._tensors = k_codes, v_codes, k_scales, v_scales   # held, as their addresses are below
         self.layers, self.pages, self.kv_heads, self.head_dim = layers, pages, kv_heads, dim
         self.block_size = units * UNIT
         self.device = k_codes.device
         self._layers = [ctypes.byref(nat.Kv8Cache(nat.ptr(k_codes[i]), nat.ptr(v_codes[i]), nat.ptr(k_scales[i]),
                                                   nat.ptr(v_scales[i]), pages, kv_heads, dim, self.block_size))
                         for i in range(layers)]
+
+    k_codes = property(lambda self: self._tensors[0])
+    v_codes = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
 
     @classmethod
     def allocate(cls, *, layers: int, blocks: int, kv_heads: int, head_dim: int = 128, block_size: int = 64,
@@ -199,11 +211,9 @@ class PagedKVCache:
         self._slots(slots)
         if key.shape[0] != slots.shape[0] or value.shape[0] != slots.shape[0]:
             raise ValueError("key, value and slots must have as many tokens")
-        with torch.cuda.device(self.device):
-            rc = nat.lib().tq_kv8_append(self._layer(layer), nat.ptr(key), key.stride(0), key.stride(1), nat.ptr(value),
-                                         value.stride(0), value.stride(1), nat.dtype_code(key.dtype), nat.ptr(slots),
-                                         slots.shape[0], nat.stream_handle(self.device))
-        nat.check(rc, "tq_kv8_append")
+        nat.launch(self.device, "tq_kv8_append", nat.lib().tq_kv8_append, self._layer(layer), key.data_ptr(),
+                   key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+                   nat.dtype_code(key.dtype), slots.data_ptr(), slots.shape[0])
 
     def read(self, layer: int, slots: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values [n, kv_heads, head_dim] of ``slots`` [n] in ``dtype``; zeros for slots outside the cache."""
@@ -211,11 +221,10 @@ class PagedKVCache:
         self._slots(slots)
         code = nat.dtype_code(dtype)
         out = torch.empty((2, slots.shape[0], self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        k, v = out[0], out[1]
-        with torch.cuda.device(self.device):
-            rc = nat.lib().tq_kv8_read(self._layer(layer), nat.ptr(slots), slots.shape[0], code, nat.ptr(k), k.stride(0),
-                                       k.stride(1), nat.ptr(v), v.stride(0), v.stride(1), nat.stream_handle(self.device))
-        nat.check(rc, "tq_kv8_read")
+        k, v = out.unbind(0)
+        row, head = self.kv_heads * self.head_dim, self.head_dim
+        nat.launch(self.device, "tq_kv8_read", nat.lib().tq_kv8_read, self._layer(layer), slots.data_ptr(),
+                   slots.shape[0], code, k.data_ptr(), row, head, v.data_ptr(), row, head)
         return k, v
 
     def attend(self, layer: int, query: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *, scale: float,
@@ -262,11 +271,9 @@ class PagedKVCache:
             workspace = paged_attention_workspace(tokens, batch, hq, self.kv_heads, dim, max_query, bound, self.device)
         elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != self.device:
             raise ValueError(f"workspace must be contiguous fp32 on {self.device}")
-        with torch.cuda.device(self.device):
-            rc = nat.lib().tq_kv8_attention(
-                self._layer(layer), nat.ptr(query), query.stride(0), query.stride(1), nat.dtype_code(query.dtype),
-                nat.ptr(block_table), max(block_table.stride(0), width), width, nat.ptr(lengths), nat.ptr(query_start),
-                tokens, batch, hq, max_query, bound, float(scale), nat.ptr(out), out.stride(0), out.stride(1),
-                nat.ptr(workspace), workspace.numel() if workspace is not None else 0, nat.stream_handle(self.device))
-        nat.check(rc, "tq_kv8_attention")
+        nat.launch(self.device, "tq_kv8_attention", nat.lib().tq_kv8_attention,
+                   self._layer(layer), query.data_ptr(), query.stride(0), query.stride(1), nat.dtype_code(query.dtype),
+                   block_table.data_ptr(), max(block_table.stride(0), width), width, lengths.data_ptr(),
+                   nat.ptr(query_start), tokens, batch, hq, max_query, bound, float(scale), out.data_ptr(), out.stride(0),
+                   out.stride(1), nat.ptr(workspace), workspace.numel() if workspace is not None else 0)
         return out

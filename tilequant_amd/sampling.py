@@ -7,6 +7,7 @@ synchronisation, so it can be captured behind a model's logits.  The rules are i
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Union
 
 import torch
@@ -16,6 +17,11 @@ from . import _native as nat
 Setting = Union[float, int, torch.Tensor]
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+@lru_cache(maxsize=1024)
+def _workspace_elems(rows: int, vocab: int) -> int:
+    return int(nat.lib().tq_sample_workspace_elems(rows, vocab))
 
 
 def _setting(name: str, value: Setting, dtype: torch.dtype, logits: torch.Tensor):
@@ -60,11 +66,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
     elif out.dtype != torch.int64 or out.shape != (rows,) or not out.is_contiguous() or out.device != logits.device:
         raise ValueError("out must be a contiguous int64 vector with one entry per row on the logits' device")
     # scratch of this call alone: calls on other streams, and graphs, have their own
-    elems = int(nat.lib().tq_sample_workspace_elems(rows, vocab))
+    elems = _workspace_elems(rows, vocab)
     workspace = torch.empty((elems,), dtype=torch.int64, device=logits.device) if elems else None
-    with torch.cuda.device(logits.device):
-        rc = nat.lib().tq_sample_tokens(
-            logits.data_ptr(), logits.stride(0), code, rows, vocab, uniform.data_ptr(), t, float(t_all), k, int(k_all), p,
-            float(p_all), m, float(m_all), out.data_ptr(), nat.ptr(workspace), elems, nat.stream_handle(logits.device))
-    nat.check(rc, "tq_sample_tokens")
+    nat.launch(logits.device, "tq_sample_tokens", nat.lib().tq_sample_tokens,
+               logits.data_ptr(), logits.stride(0), code, rows, vocab, uniform.data_ptr(), t, float(t_all), k, int(k_all),
+               p, float(p_all), m, float(m_all), out.data_ptr(), nat.ptr(workspace), elems)
     return out
