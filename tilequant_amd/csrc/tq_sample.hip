@@ -79,6 +79,7 @@ struct SampleArgs {
 struct F32In {
   using T = float;
   static constexpr int kVec = 4;
+  static constexpr int kLow = 0;   // low bits of a logit's key that are the same for all of one sign
   __device__ static inline float shift(u32x4& w) {   // the first element, the others one place down
     const float f = __uint_as_float(w[0]);
     w[0] = w[1];
@@ -95,6 +96,7 @@ template <class XT>
 struct H16In {
   using T = uint16_t;
   static constexpr int kVec = 8;
+  static constexpr int kLow = std::is_same<XT, Bf16>::value ? 16 : 13;
   __device__ static inline float shift(u32x4& w) {
     const float f = XT::to_f32((uint16_t)(w[0] & 0xffffu));
     w[0] = (w[0] >> 16) | (w[1] << 16);
@@ -600,7 +602,9 @@ __device__ __forceinline__ void fill_bins(const typename IN::T* row, int vocab, 
 
 // Where a search stops in the row, its bins being known.  The tokens of the bin are narrowed down, 64 ranges of their
 // order (key, then index) at a time: over the row while they are more than the list holds, then in the list, until at
-// most kSampSort are left, which are sorted.  Each turn divides the range of 64-bit numbers by 32 or more.
+// most kSampSort are left, which are sorted.  Each turn divides the range of the numbers by 32 or more.  The numbers
+// leave out what does not vary, the low bits of a 16-bit logit's key and the high ones of the index: of a bin's several
+// thousand bf16 tokens, many of them equal, one turn leaves few enough (with 64-bit numbers five turns, 3.6 us each).
 // gathered: the list holds that many tokens, all of the bin among them, and stays as it is; or -1.
 template <class IN>
 __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab, const SampleRow& r, uint64_t* cells,
@@ -617,22 +621,27 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
   int64_t base_count = sh.row.before[b];
   uint64_t base_mass = sh.row.mass_before[b];
   int count = (int)sh.row.count[b], whole = max(gathered, 0);
+  const int index_bits = 32 - __builtin_clz((uint32_t)vocab);
+  const uint64_t index_mask = (1ull << index_bits) - 1;
+  const auto number = [&](uint64_t entry) {
+    return (entry >> (32 + IN::kLow)) << index_bits | (entry & index_mask);
+  };
   // the range of the order that the bin takes up, a little wide: place says what is in it
-  uint64_t first = 0, last = ~0ull;
+  uint64_t first = 0, last = number(~0ull);
   const float upper = 2.0f * (r.half_top - from / r.step), lower = 2.0f * (r.half_top - to / r.step);
   const float slack = 1e-5f * (fabsf(upper) + fabsf(lower) + fabsf(r.top));
   if (upper + slack < FLT_MAX && lower - slack > -FLT_MAX) {
-    first = (uint64_t)~key_of(upper + slack) << 32;
-    last = (uint64_t)~key_of(lower - slack) << 32 | 0xffffffffull;
+    first = number((uint64_t)~key_of(upper + slack) << 32);
+    last = number((uint64_t)~key_of(lower - slack) << 32 | 0xffffffffull);
   }
   bool listed = gathered >= 0;
-  const auto in = [&](float v, uint64_t e) {
+  const auto in = [&](float v, uint64_t x) {
     const float place = r.place(v);
-    return place >= from && place < to && e >= first && e <= last;
+    return place >= from && place < to && x >= first && x <= last;
   };
-  for (int turn = 0; turn < 20; ++turn) {   // 64 bits, 5 or more a turn, and one turn to list them
+  for (int turn = 0; turn < 20; ++turn) {   // up to 51 bits, 5 or more a turn, and one turn to list them
     if (!listed && count <= kSampList) {
-      collect<IN>(row, vocab, r, list, sh, in);
+      collect<IN>(row, vocab, r, list, sh, [&](float v, uint64_t e) { return in(v, number(e)); });
       whole = min(sh.n_list, kSampList);
       listed = true;
     }
@@ -646,14 +655,14 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
     if (listed) {
 #pragma unroll 1
       for (int i = t; i < whole; i += kSampThreads) {
-        const uint64_t e = list[i];
+        const uint64_t e = list[i], x = number(e);
         const float v = logit_of(e);
-        if (in(v, e)) add_to_cell(&mine[(int)((e - first) >> shift) * cols], r.weight(v));
+        if (in(v, x)) add_to_cell(&mine[(int)((x - first) >> shift) * cols], r.weight(v));
       }
     } else {
       each_token<IN>(row, vocab, t, row_vectors<IN>(row, vocab), kSampThreads, [&](float z, int i) {
         const float v = r.see(z);
-        const uint64_t x = entry_of(v, i);
+        const uint64_t x = number(entry_of(v, i));
         if (in(v, x)) add_to_cell(&mine[(int)((x - first) >> shift) * cols], r.weight(v));
       });
     }
@@ -667,11 +676,6 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
     first += (uint64_t)w << shift;
     const uint64_t end = first + ((1ull << shift) - 1);
     last = end < last ? end : last;
-    const uint64_t end_of_key = first | 0xffffffffull;   // the rest of one key's indexes is empty
-    if (last <= end_of_key) {
-      const uint64_t most = (first & ~0xffffffffull) | (uint64_t)(uint32_t)vocab;
-      last = most < last ? most : last;
-    }
     __syncthreads();   // the next turn writes the bins
   }
   __syncthreads();   // every thread has read the list's length
@@ -679,7 +683,7 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
   __syncthreads();
   for (int i = t; i < whole; i += kSampThreads) {
     const uint64_t e = list[i];
-    if (in(logit_of(e), e)) {
+    if (in(logit_of(e), number(e))) {
       const int at = atomicAdd(&sh.n_work, 1);
       if (at < kSampSort) work[at] = e;
     }
