@@ -259,16 +259,25 @@ __device__ inline uint64_t block_before(uint64_t v, uint64_t* red) {
 }
 
 // f(z, i) for the vectors vec0, vec0 + step, .. of the row: 16-byte aligned loads from the one that holds the row's first
-// element on; what they hold beside the row is given as -infinity with an index out of range.
+// element on; what they hold beside the row is given as -infinity with an index out of range.  kBatch vectors are loaded
+// while the batch before is looked at.
 template <class IN, int kBatch, class F>
 __device__ __forceinline__ void sweep(const typename IN::T* row, int vocab, int vec0, int vec1, int step, F f) {
   constexpr int V = IN::kVec;
   const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(typename IN::T));
   const u32x4* base = reinterpret_cast<const u32x4*>(row - off);
+  if (vec0 >= vec1) return;
+  u32x4 next[kBatch];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) next[b] = base[min(vec0 + b * step, vec1 - 1)];
+#pragma unroll 1
   for (int j0 = vec0; j0 < vec1; j0 += step * kBatch) {
     u32x4 w[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) w[b] = base[min(j0 + b * step, vec1 - 1)];
+    for (int b = 0; b < kBatch; ++b) {
+      w[b] = next[b];
+      next[b] = base[min(j0 + (kBatch + b) * step, vec1 - 1)];
+    }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int j = j0 + b * step;
@@ -981,12 +990,16 @@ __device__ __forceinline__ void hand_over(const SampleArgs& a, int b, const type
   if (t == 0) sh.n_list = 0;
   __syncthreads();
   sweep<IN, 1>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int i0) {
+    uint32_t taken = 0;
 #pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) {
-      const float v = r.see(z[e]);
-      if (take(v)) {
-        const int at = atomicAdd(&sh.n_list, 1);
-        if (at < kChunkList) list[at] = entry_of(v, i0 + e);
+    for (int e = 0; e < IN::kVec; ++e) taken |= take(r.see(z[e])) ? 1u << e : 0u;
+    if (taken) {   // places for all of the vector's at once
+      int at = atomicAdd(&sh.n_list, __builtin_popcount(taken));
+#pragma unroll
+      for (int e = 0; e < IN::kVec; ++e) {
+        if (!(taken >> e & 1u)) continue;
+        if (at < kChunkList) list[at] = entry_of(r.see(z[e]), i0 + e);
+        ++at;
       }
     }
   });
