@@ -154,6 +154,21 @@ def test_odd_settings(vocab):
     check(z, torch.tensor([0.0, 1.0, 1.5, 0.0, 1.0, 1.0, 0.0]), exact=True, k=20)
 
 
+@pytest.mark.parametrize("setting", [dict(), dict(temperature=0.0), dict(temperature=float("nan")), dict(top_k=1), dict(top_k=40),
+                                     dict(top_k=512), dict(top_k=513), dict(top_k=10 ** 12), dict(top_k=-3), dict(min_p=0.05),
+                                     dict(top_p=0.8), dict(top_p=0.8, min_p=0.01), dict(top_k=300, top_p=0.9, min_p=0.02),
+                                     dict(temperature=0.0, top_k=40, top_p=0.5)])
+@pytest.mark.parametrize("vocab", [400, 40000])
+def test_numbers_for_all_rows_equal_vectors(vocab, setting):
+    z, u = logits_like(9, vocab, torch.bfloat16, seed=vocab + 1)
+    z[3], z[4, ::2], z[5, 7] = -float("inf"), float("nan"), float("inf")
+    z, u = z.to(DEV), u.to(DEV)
+    types = dict(temperature=torch.float32, top_k=torch.int32, top_p=torch.float32, min_p=torch.float32)
+    vectors = {n: torch.full((9,), min(v, 2 ** 31 - 1) if n == "top_k" else v, dtype=types[n], device=DEV)
+               for n, v in setting.items()}
+    assert torch.equal(sample_tokens(z, u, **setting), sample_tokens(z, u, **vectors))
+
+
 def test_strides_and_alignment():
     """Views with odd row strides and odd first elements, and an output that the caller holds."""
     base = torch.randn((6, 1111), generator=torch.Generator().manual_seed(4)) * 3

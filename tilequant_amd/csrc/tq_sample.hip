@@ -21,7 +21,7 @@
 //          the bins where a target falls are looked at: they are narrowed down by key and index until at most 256 are
 //          left to sort.  Bins have 16 or more columns, and a lane adds to the column of its number: no bank conflicts, no
 //          two lanes at one address.
-// Short rows take one launch of one workgroup per row.  Others are cut in C chunks, and there are four:
+// Short rows take one launch of one workgroup per row.  Others are cut in C chunks, and there are up to four:
 // maxima of every chunk; the chunk's list or bins, now that the row's maximum is known; the tokens of the bins that the
 // row's searches can end in, which the bins' sums tell, gathered; and one workgroup per row that finishes from the list
 // in LDS.  Masses being integers, C does not change the answer.
@@ -40,12 +40,13 @@ constexpr int kChunkCols = 16;
 constexpr int kChunkList = 2048;       // list entries that one chunk may hand over
 constexpr int kMaxima = 2048;          // maxima of a row, at most
 constexpr int kSampList = 8192;        // entries of the sorted list: 8 bytes of key and index, 8 of prefix mass
-constexpr int kSampTopK = 512;         // largest k of the list path: half the threads' maxima
-constexpr int kSampSort = kSampThreads / 4;   // entries sorted by rank
+constexpr int kSampTopK = 512;         // largest k of the list path
+constexpr int kSampSort = 512;         // entries sorted by rank, an entry a thread at most
+constexpr int kSampEnd = 256;          // a search's last entries: a turn more costs as much as sorting twice as many
 constexpr int kSampBoundBins = 512;
 constexpr int kSampMaxVocab = 500000;  // a column's count has 13 bits: at most 8191 tokens of a row per column
 constexpr int kChunkMost = 120000;     // tokens of a chunk, for the same reason
-constexpr int kSampWhole = 2048;       // the bins down to the last one needed are sorted together up to this many tokens
+constexpr int kSampWhole = 512;        // the bins down to the last one needed are sorted together up to this many tokens
 constexpr uint64_t kSampCount = 1ull << 51;    // one token in a column's word: count from bit 51 on, mass below
 
 struct SampleArgs {
@@ -369,18 +370,20 @@ __device__ __forceinline__ Best argmax_row(const typename IN::T* row, int vocab,
 __device__ inline uint64_t entry_of(float z, int i) { return (uint64_t)~key_of(z) << 32 | (uint32_t)i; }
 __device__ inline float logit_of(uint64_t entry) { return of_key(~(uint32_t)(entry >> 32)); }
 
-// Sorts n entries; up to kSampSort by rank (four threads per entry, each against a quarter of the others, through spare),
-// more in a bitonic network.
+// Sorts n entries; up to kSampSort by rank (kSampThreads / n threads per entry, up to 4, each against a part of the
+// others, through spare), more in a bitonic network.
 __device__ __forceinline__ void sort_small(uint64_t* list, uint64_t* spare, int n) {
-  const int t = threadIdx.x, e = t >> 2, part = t & 3;
+  const int t = threadIdx.x;
+  const int parts = n <= kSampThreads / 4 ? 4 : n <= kSampThreads / 2 ? 2 : 1;
+  const int e = t / parts, part = t & (parts - 1);
   uint64_t mine = ~0ull;
   int rank = 0;
   if (e < n) {
     mine = list[e];
-    for (int j = part; j < n; j += 4) rank += list[j] < mine;
+#pragma unroll 8
+    for (int j = part; j < n; j += parts) rank += list[j] < mine;
   }
-  rank += __shfl_xor(rank, 1);
-  rank += __shfl_xor(rank, 2);
+  for (int o = 1; o < parts; o <<= 1) rank += __shfl_xor(rank, o);
   if (e < n && part == 0) spare[rank] = mine;
   __syncthreads();
   if (t < n) list[t] = spare[t];
@@ -611,7 +614,7 @@ __device__ __forceinline__ void fill_bins(const typename IN::T* row, int vocab, 
 
 // Where a search stops in the row, its bins being known.  The tokens of the bin are narrowed down, 64 ranges of their
 // order (key, then index) at a time: over the row while they are more than the list holds, then in the list, until at
-// most kSampSort are left, which are sorted.  Each turn divides the range of the numbers by 32 or more.  The numbers
+// most kSampEnd are left, which are sorted.  Each turn divides the range of the numbers by 32 or more.  The numbers
 // leave out what does not vary, the low bits of a 16-bit logit's key and the high ones of the index: of a bin's several
 // thousand bf16 tokens, many of them equal, one turn leaves few enough (with 64-bit numbers five turns, 3.6 us each).
 // gathered: the list holds that many tokens, all of the bin among them, and stays as it is; or -1.
@@ -624,7 +627,7 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
   uint64_t* work = cells + kSampList;   // the turns' cells; then the last entries, a copy and their prefix masses
   constexpr int kRowCols = 128;         // a column counts up to 8191 tokens: of the whole row, and of the list
   constexpr int kListCols = 32;
-  static_assert(kWorkBins * kRowCols == kSampList && 3 * kSampSort <= kSampList, "what the second half holds");
+  static_assert(kWorkBins * kRowCols == kSampList && 3 * kSampEnd <= kSampList, "what the second half holds");
   const int b = bin_of_search(s, sh.row, 0, 0);
   const float from = (float)b, to = (float)(b + 1);
   int64_t base_count = sh.row.before[b];
@@ -654,7 +657,7 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
       whole = min(sh.n_list, kSampList);
       listed = true;
     }
-    if (listed && count <= kSampSort) break;
+    if (listed && count <= kSampEnd) break;
     const uint64_t range = last - first;
     const int shift = max(0, 58 - (int)__builtin_clzll(range | 1));
     const int cols = listed ? kListCols : kRowCols;
@@ -694,13 +697,13 @@ __device__ __forceinline__ Found search_row(const typename IN::T* row, int vocab
     const uint64_t e = list[i];
     if (in(logit_of(e), number(e))) {
       const int at = atomicAdd(&sh.n_work, 1);
-      if (at < kSampSort) work[at] = e;
+      if (at < kSampEnd) work[at] = e;
     }
   }
   __syncthreads();
-  const int n = max(1, min(sh.n_work, kSampSort));
-  uint64_t* prefix = work + 2 * kSampSort;
-  sort_small(work, work + kSampSort, n);
+  const int n = max(1, min(sh.n_work, kSampEnd));
+  uint64_t* prefix = work + 2 * kSampEnd;
+  sort_small(work, work + kSampEnd, n);
   sum_list(work, prefix, n, r, sh);
   int at = s.by_rank ? (int)(s.rank - base_count) : first_past(prefix, n, base_mass, s.least);
   at = max(min(at, n - 1), 0);
@@ -1228,8 +1231,12 @@ static int sample_launch(SampleArgs a, const SamplePlan& p, uint64_t* ws, hipStr
   TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_finish_kernel<IN>>(lds)));
   const dim3 grid(p.chunks, a.rows), block(kChunkThreads);
   hipLaunchKernelGGL(sample_max_kernel<IN>, grid, block, 0, s, a);
-  hipLaunchKernelGGL(sample_chunk_kernel<IN>, grid, block, 0, s, a);
-  hipLaunchKernelGGL(sample_gather_kernel<IN>, grid, block, 0, s, a);
+  // what no row of the call has to do, where one number sets all rows
+  const bool greedy = !a.temperature && !(a.temperature0 > 0.0f);
+  const int k = a.top_k0 < a.vocab ? a.top_k0 : 0;
+  const bool lists = !a.top_k && (k > 0 ? k <= kSampTopK : !a.top_p && !a.min_p && a.top_p0 >= 1.0f && a.min_p0 > 0.0f);
+  if (!greedy) hipLaunchKernelGGL(sample_chunk_kernel<IN>, grid, block, 0, s, a);
+  if (!greedy && !lists) hipLaunchKernelGGL(sample_gather_kernel<IN>, grid, block, 0, s, a);
   hipLaunchKernelGGL(sample_finish_kernel<IN>, dim3(a.rows), dim3(kSampThreads), lds, s, a);
   return (int)hipGetLastError();
 }

@@ -69,6 +69,6 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: S
     elems = _workspace_elems(rows, vocab)
     workspace = torch.empty((elems,), dtype=torch.int64, device=logits.device) if elems else None
     nat.launch(logits.device, "tq_sample_tokens", nat.lib().tq_sample_tokens,
-               logits.data_ptr(), logits.stride(0), code, rows, vocab, uniform.data_ptr(), t, float(t_all), k, int(k_all),
+               logits.data_ptr(), logits.stride(0), code, rows, vocab, uniform.data_ptr(), t, float(t_all), k, min(max(int(k_all), 0), vocab),
                p, float(p_all), m, float(m_all), out.data_ptr(), nat.ptr(workspace), elems)
     return out
