@@ -122,19 +122,24 @@ __device__ inline uint32_t key_of(float z) {
 }
 __device__ inline float of_key(uint32_t k) { return __uint_as_float(k ^ ((int32_t)k < 0 ? 0x80000000u : 0xffffffffu)); }
 
-// 2^x for x in [-42, 0]: the Taylor series of e^(f ln 2), |f| <= 1/2, to degree 11 (6e-15 relative).
-__device__ inline double exp2_small(double x) {
+// 2^x for x in [-42, 0]: the Taylor series of e^(f ln 2), |f| <= 1/2, to degree 11 (6e-15 relative).  Its coefficients are
+// made scalar operands: held in vector registers, each step would begin with a copy of one.
+__device__ __forceinline__ double in_scalar(double c) {
+  asm("" : "+s"(c));
+  return c;
+}
+__device__ __forceinline__ double exp2_small(double x) {
   const double n = __builtin_rint(x);
   const double f = (x - n) * 0.693147180559945309417;
-  double r = 1.0 / 39916800.0;
-  r = fma(r, f, 1.0 / 3628800.0);
-  r = fma(r, f, 1.0 / 362880.0);
-  r = fma(r, f, 1.0 / 40320.0);
-  r = fma(r, f, 1.0 / 5040.0);
-  r = fma(r, f, 1.0 / 720.0);
-  r = fma(r, f, 1.0 / 120.0);
-  r = fma(r, f, 1.0 / 24.0);
-  r = fma(r, f, 1.0 / 6.0);
+  double r = in_scalar(1.0 / 39916800.0);
+  r = fma(r, f, in_scalar(1.0 / 3628800.0));
+  r = fma(r, f, in_scalar(1.0 / 362880.0));
+  r = fma(r, f, in_scalar(1.0 / 40320.0));
+  r = fma(r, f, in_scalar(1.0 / 5040.0));
+  r = fma(r, f, in_scalar(1.0 / 720.0));
+  r = fma(r, f, in_scalar(1.0 / 120.0));
+  r = fma(r, f, in_scalar(1.0 / 24.0));
+  r = fma(r, f, in_scalar(1.0 / 6.0));
   r = fma(r, f, 0.5);
   r = fma(r, f, 1.0);
   r = fma(r, f, 1.0);
@@ -1045,17 +1050,26 @@ sample_chunk_kernel(SampleArgs a) {
   uint64_t* own = cells + (t & (kChunkCols - 1));
   uint64_t above = 0, above_mass = 0;
   sweep<IN, 1>(row, a.vocab, v0 + t, v1, kChunkThreads, [&](const auto& z, int) {
+    // two tokens' weights at a time, wanted or not: a weight alone is a chain of 20 dependent instructions
 #pragma unroll
-    for (int e = 0; e < IN::kVec; ++e) {
-      const float v = r.see(z[e]), place = r.place(v);
-      if (SampleRow::alive(place)) {
-        const double w = exp2_small(r.log2_weight(v));
-        if (set.m > 0.0 && w >= set.m) {
-          above += 1;
-          above_mass += SampleRow::mass(w);
-        }
-        add_to_cell(&own[(int)place * kChunkCols], w);
+    for (int e = 0; e < IN::kVec; e += 2) {
+      float place[2];
+      double w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float v = r.see(z[e + i]);
+        place[i] = r.place(v);
+        w[i] = exp2_small(r.log2_weight(SampleRow::alive(place[i]) ? v : r.top));
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (SampleRow::alive(place[i])) {
+          if (set.m > 0.0 && w[i] >= set.m) {
+            above += 1;
+            above_mass += SampleRow::mass(w[i]);
+          }
+          add_to_cell(&own[(int)place[i] * kChunkCols], w[i]);
+        }
     }
   });
   above = block_sum<kChunkThreads>(above, sh.red_u);   // and the barrier after the cells' additions
