@@ -488,6 +488,7 @@ kv8_append_kernel(AppendArgs a) {
 // code * scale, rounded once, of the listed slots (slots outside the cache: zeros).  One wave per 16 list entries,
 // head and K or V.  Keys are copied row by row; values, stored transposed, unit by unit: the wave takes the unit of its
 // first entry not yet written, and with it every entry of that unit (a list in token order has one or two units).
+// The bound is memory: 8192 tokens, 8 kv heads of 128: 50 MB in 10 us, as fast as a large copy.
 struct ReadArgs {
   const int32_t* slots;
   const int8_t* codes[2];

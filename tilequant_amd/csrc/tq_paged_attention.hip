@@ -22,6 +22,8 @@
 // O^T = V^T P^T as they stand.  For that, row r = 4 u + v of the A block m holds key 16 u + 4 m + v of the 64-key tile.
 #include "tq_common.h"
 
+#include <float.h>
+
 namespace tq {
 
 constexpr float kLog2e8 = 1.4426950408889634f;
@@ -196,9 +198,11 @@ __device__ __forceinline__ float softmax_tile(v4f (&s)[4], bool live, int nv, fl
       for (int v = 0; v < 4; ++v) s[m][v] = 4 * m + v < nv ? s[m][v] : -3.0e38f;
     live = live && nv > 0;
   }
-  float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+  // three at a time: 8 instructions, where a tree of pairs makes 20, each of whose leaves is first made canonical
+  float top = s[0][0];
 #pragma unroll
-  for (int m = 1; m < 4; ++m) top = fmaxf(top, fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3])));
+  for (int j = 1; j < 15; j += 2) top = fmaxf(fmaxf(top, s[j >> 2][j & 3]), s[(j + 1) >> 2][(j + 1) & 3]);
+  top = fmaxf(fmaxf(top, s[3][3]), -FLT_MAX);
   const float mine = live ? fmaf(top, f, vs.log) : -INFINITY;
   const float M = fmaxf(sm.M, g4_max(mine));
   const float ref = M == -INFINITY ? 0.0f : M;
@@ -227,6 +231,7 @@ __device__ __forceinline__ float softmax_tile(v4f (&s)[4], bool live, int nv, fl
 // Workgroup (split, sequence x kv head, row tile): NW waves take the split's 64-key tiles in turn, each with a running
 // softmax of its own over 16 query rows; a tile's codes go straight from memory to the wave that multiplies them (K: 8,
 // V: 8 16-byte loads per lane at D = 128).  The waves' results are joined through LDS in wave order.
+// The bound is memory: 4 sequences of 131072 tokens, 8 kv heads of 128, 1.08 GB: 188 us, 5.7 TB/s.
 template <class XT, int D, int NW>
 __global__ void __launch_bounds__(NW * kWave)
 kv8_split_kernel(Kv8Args a) {
@@ -355,6 +360,10 @@ kv8_split_kernel(Kv8Args a) {
 // Workgroup (sequence x kv head, row tile, split): four waves of 32 query rows each over 64-key tiles.  The four waves
 // widen a tile's codes once, a quarter each, into LDS in operand order (1 KiB per operand, lane after lane: no bank
 // conflicts either way), two tiles deep, and every wave multiplies its rows with all of them.
+// The bound is instruction issue, two waves a SIMD: matrix instructions take 30% of the SIMDs' cycles, the vector
+// instructions (per tile and wave 170 of softmax, 32 of them exponentials, and 85 of widening) 52%.  4 prompts of 1500 to
+// 2048 tokens, 24 / 8 heads of 128: 137 us, 0.61 PFLOP/s of what the mask leaves; 512 tokens over 16384: 0.74; a large
+// fp16 product reaches 1.19.  48 rows a wave, or the next tile's scores beside this tile's softmax, spill (203 us and more).
 constexpr int kKv8Block = 128;   // rows per workgroup
 constexpr int kKv8Waves = 4;
 
@@ -374,7 +383,7 @@ kv8_block_kernel(Kv8Args a) {
   const Kv8Seq sq = kv8_seq(a, b);
   const int rows = sq.n * a.G;
   // The last row tiles have the most keys: they go first, over all sequences and heads (4 prompts of up to 2048
-  // tokens, 8 kv heads: 143 us, 173 with all tiles of a head before the next head's).
+  // tokens, 8 kv heads: 143 us when this was tried, 173 with all tiles of a head before the next head's).
   const int tiles = (rows + kKv8Block - 1) / kKv8Block;
   const int tile = tiles - 1 - (int)blockIdx.y;
   if (tile < 0) return;
@@ -455,18 +464,31 @@ kv8_block_kernel(Kv8Args a) {
       __syncthreads();   // the tile is staged; nobody reads the other buffer any more
       const bool more = base + kKv8Tile < key1;
       if (more) fetch(base + kKv8Tile);
+      // Operands are read once for both row blocks, a group ahead of the products that take them: the scheduling
+      // barriers keep the compiler from moving the reads down to their use, where each product waits for LDS (512 tokens
+      // over 16384, 24 / 8 heads: 137 us against 141).
       v4f s[2][4];
+      v4i kk[2][KS];
+#pragma unroll
+      for (int i = 0; i < KS; ++i) kk[0][i] = kl[(buf * KO + i) * kWave + lane];
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
+        if (m < 3) {
+#pragma unroll
+          for (int i = 0; i < KS; ++i) kk[(m + 1) & 1][i] = kl[(buf * KO + (m + 1) * KS + i) * kWave + lane];
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < 2; ++x) s[x][m] = v4f{qr[x].bias, qr[x].bias, qr[x].bias, qr[x].bias};
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {   // an operand is read once for both row blocks
-          const v4i kk = kl[(buf * KO + m * KS + i) * kWave + lane];
+        for (int i = 0; i < KS; ++i)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) s[x][m] = mfma16<Fp16>(kk, qr[x].op[i], s[x][m]);
-        }
+          for (int x = 0; x < 2; ++x) s[x][m] = mfma16<Fp16>(kk[m & 1][i], qr[x].op[i], s[x][m]);
       }
+      v4i vv[2][4];   // of two dimension blocks; the first are read under the softmax
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vv[0][i] = vl[(buf * VO + i) * kWave + lane];
+      __builtin_amdgcn_sched_barrier(0);
       v4i p[2][2];
       float alpha[2];
       bool moved = false;
@@ -489,13 +511,18 @@ kv8_block_kernel(Kv8Args a) {
             for (int v = 0; v < 4; ++v) o[x][d][v] *= alpha[x];
       }
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const v4i v0 = vl[(buf * VO + 2 * d) * kWave + lane], v1 = vl[(buf * VO + 2 * d + 1) * kWave + lane];
+      for (int d = 0; d < DB; d += 2) {
+        if (d + 2 < DB) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          o[x][d] = mfma16<Fp16>(v0, p[x][0], o[x][d]);
-          o[x][d] = mfma16<Fp16>(v1, p[x][1], o[x][d]);
+          for (int i = 0; i < 4; ++i) vv[(d / 2 + 1) & 1][i] = vl[(buf * VO + 2 * (d + 2) + i) * kWave + lane];
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) o[x][d + e] = mfma16<Fp16>(vv[(d / 2) & 1][2 * e + k], p[x][k], o[x][d + e]);
       }
       buf ^= 1;
       if (more) stage(buf);
@@ -538,7 +565,8 @@ kv8_block_kernel(Kv8Args a) {
 
 // ---- joining the splits ----------------------------------------------------------
 //
-// One wave per (token, query head), splits in order, eight at a time so that their loads go out together.
+// One wave per (token, query head), splits in order, eight at a time so that their loads go out together: 4 us for 32
+// tokens of 28 heads in up to 17 splits, about an empty launch.
 template <class XT, int D>
 __global__ void __launch_bounds__(256)
 kv8_merge_kernel(Kv8Args a) {
