@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-enum { TQ_DTYPE_BF16 = 0, TQ_DTYPE_FP16 = 1, TQ_DTYPE_FP32 = 2 /* tq_quant_tensor_absmax only */ };
+enum { TQ_DTYPE_BF16 = 0, TQ_DTYPE_FP16 = 1, TQ_DTYPE_FP32 = 2 /* tq_quant_tensor_absmax, tq_sample_tokens */ };
 
 /* Storage order of the 64x64 elements inside one packed tile.
  * ROW_MAJOR: tile[j][k] at j*64+k (the reference packer's order, pack.py:115-175).

@@ -14,10 +14,16 @@ Module map (reference file -> this package):
   src/models/mixed_linear.py                   -> mixed_linear
   src/models/rules.py                          -> rules
   src/quantization/types.py                    -> types
+
+For serving ragged requests, with no reference counterpart: ``paged_cache`` (block
+tables, a paged INT8 KV cache and attention over it) and ``sampling``.
 """
 from __future__ import annotations
 
 __all__ = [
+    "BlockTables",
+    "PagedKVCache",
+    "sample_tokens",
     "Pack",
     "MixedLinear",
     "MixedLinearGroup",
@@ -33,8 +39,10 @@ __all__ = [
 from .gemm_rows_splitk_64x64 import gemm_mixed_rows_splitk
 from .mixed_linear import MixedLinear, MixedLinearGroup, MixedLinearSlice, fuse_projection_groups
 from .pack import Pack, pack_weight_from_tile_ids
+from .paged_cache import BlockTables, PagedKVCache
 from .quant_utils import (
     activation_tile_absmax_scales,
     quantize_activation_tile_absmax,
     quantize_activation_tile_with_scales,
 )
+from .sampling import sample_tokens
