@@ -535,7 +535,7 @@ int tq_kv8_read(const tq_kv8_cache* cache, const int32_t* slots, int n, int dtyp
  * the cache are left out; q rows of no sequence, and queries past max_query of
  * their sequence, leave out as it was.  q, out: [tokens, q_heads, head_dim] with
  * strides per token / head, 16-byte aligned, strides multiples of 8; at most 128
- * query heads per kv head.  fp32 accumulation.  workspace =
+ * query heads per kv head; batch * kv_heads <= 65535.  fp32 accumulation.  workspace =
  * tq_kv8_attention_workspace_elems() floats, 8-byte aligned (0: none needed). */
 int64_t tq_kv8_attention_workspace_elems(int tokens, int batch, int q_heads, int kv_heads, int head_dim,
                                          int max_query, int max_len);

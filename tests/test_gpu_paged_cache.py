@@ -215,6 +215,21 @@ def test_append_long_lists_of_mixed_runs(dim, heads, tokens):
     c.check()
 
 
+def test_sizes_that_do_not_fit_and_rows_that_overlap():
+    lengths, news = [40, 70], [3, 5]
+    c, table, q, starts, scale = attention_case(lengths, news, 4, 2, 64, 16, torch.bfloat16, seed=5)
+    want = run(c, table, lengths, q, starts, scale)
+    table, lengths, starts = i32(table), i32(lengths), i32(starts)
+    got = c.gpu.attend(1, q.to(DEV), table, lengths, scale=scale, query_start=starts, max_query=2 ** 32 + 1)
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError, match="overlap"):      # one row for all sequences
+        c.gpu.attend(1, q.to(DEV), table[:1].expand(2, -1), lengths, scale=scale, query_start=starts, max_query=5)
+    t = TablesPair(2, 2, 4, 16)
+    for most in (-1, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="max_tokens"):
+            t.gpu.step(i32([1, 1]), max_tokens=most)
+
+
 def test_the_tensors_stay_the_objects_own():
     c, t = Cache(2, 1, 64, 16), TablesPair(2, 2, 4, 16)
     for obj, name in ((c.gpu, "k_codes"), (c.gpu, "v_scales"), (t.gpu, "lengths"), (t.gpu, "block_table")):

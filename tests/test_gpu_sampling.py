@@ -169,6 +169,17 @@ def test_numbers_for_all_rows_equal_vectors(vocab, setting):
     assert torch.equal(sample_tokens(z, u, **setting), sample_tokens(z, u, **vectors))
 
 
+@pytest.mark.parametrize("vocab", [50, 30000])
+def test_numbers_far_outside_give_the_ends(vocab):
+    """Below 0: the first kept token, 1 and above: the last, however large."""
+    z, _ = logits_like(8, vocab, torch.float32, seed=3)
+    z = z[:1].expand(8, -1).contiguous()
+    u = torch.tensor([0.0, -1.0, -float("inf"), float("nan"), 1.0, 1e9, 3e38, float("inf")])
+    for setting in (dict(top_k=20), dict(top_p=0.7), dict()):
+        got = sample_tokens(z.to(DEV), u.to(DEV), **setting).tolist()
+        assert got[:4] == got[:1] * 4 and got[4:] == got[4:5] * 4 and got[0] == int(z[0].argmax())
+
+
 def test_strides_and_alignment():
     """Views with odd row strides and odd first elements, and an output that the caller holds."""
     base = torch.randn((6, 1111), generator=torch.Generator().manual_seed(4)) * 3

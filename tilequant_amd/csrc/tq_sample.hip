@@ -442,8 +442,10 @@ struct Search {
   int64_t rank;
   uint64_t least;   // the mass from which on a search for a mass stops
   __device__ static inline Search of_rank(int64_t rank) { return Search{true, rank, 0}; }
-  __device__ static inline Search over(double target) { return Search{false, 0, (uint64_t)fmax(target, 0.0) + 1}; }
-  __device__ static inline Search from(double target) { return Search{false, 0, (uint64_t)ceil(fmax(target, 0.0))}; }
+  // masses are below 2^58 (500000 tokens); a target beyond, of a number far above 1, is as good as 2^62
+  __device__ static inline double in_range(double target) { return fmin(fmax(target, 0.0), 0x1p62); }
+  __device__ static inline Search over(double target) { return Search{false, 0, (uint64_t)in_range(target) + 1}; }
+  __device__ static inline Search from(double target) { return Search{false, 0, (uint64_t)ceil(in_range(target))}; }
   __device__ inline bool past(int64_t count, uint64_t mass) const {   // of the tokens up to and with some token
     return by_rank ? count > rank : mass >= least;
   }

@@ -110,8 +110,8 @@ class BlockTables:
             if finished.dtype not in (torch.bool, torch.uint8) or tuple(finished.shape) != (rows,) \
                     or not finished.is_contiguous() or finished.device != dev:
                 raise ValueError("finished must be a contiguous bool vector with one entry per request")
-        if max_tokens < 0:
-            raise ValueError("max_tokens must not be negative")
+        if not 0 <= max_tokens < 1 << 30:
+            raise ValueError("max_tokens must be in [0, 2^30)")
         # one allocation for the three int32 results
         out = torch.empty((2 * max_tokens + rows + 1,), dtype=torch.int32, device=dev)
         granted = torch.empty((rows,), dtype=torch.bool, device=dev)
@@ -237,7 +237,7 @@ class PagedKVCache:
         ``query_start`` there is one query per sequence; with it, queries query_start[b] .. query_start[b + 1] - 1
         are the last tokens of sequence b, causal among themselves, at most ``max_query`` of them.  A query that
         sees no key gives zeros; rows of ``out`` behind the last sequence are left as they were (a new ``out`` is
-        zeroed when ``query_start`` is given).  ``max_length``: an upper bound of the lengths (default: the
+        zeroed when ``query_start`` is given).  batch * kv_heads is at most 65535.  ``max_length``: an upper bound of the lengths (default: the
         table's width), longer ones count as that; a tight one gives the best schedule."""
         nat.require_device(query, block_table, lengths, query_start, out, workspace)
         if query.dim() != 3 or query.shape[1] % self.kv_heads:
@@ -248,11 +248,14 @@ class PagedKVCache:
                 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
             raise ValueError(f"block_table must be an int32 matrix with unit column stride on {self.device}")
         batch, width = block_table.shape
+        if batch > 1 and block_table.stride(0) < width:
+            raise ValueError("block_table rows overlap")
         _int32("lengths", lengths, (batch,), self.device)
         if query_start is not None:
             _int32("query_start", query_start, (batch + 1,), self.device)
             if max_query < 1:
                 raise ValueError("max_query must be positive")
+            max_query = min(max_query, tokens)
         elif tokens != batch or max_query != 1:
             raise ValueError("without query_start there is one query per sequence")
         bound = width * self.block_size

@@ -39,7 +39,7 @@ def _setting(name: str, value: Setting, dtype: torch.dtype, logits: torch.Tensor
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: Setting = 1.0, top_k: Setting = 0,
                   top_p: Setting = 1.0, min_p: Setting = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Token ids [rows] (int64) drawn from ``logits`` [rows, vocab] (bf16, fp16 or fp32, any row stride; vocab up to
-    500000) with one number in [0, 1) per row, ``uniform`` [rows] fp32.
+    500000, rows up to 65535) with one number in [0, 1) per row, ``uniform`` [rows] fp32.
 
     ``temperature`` (<= 0: the argmax), ``top_k`` (<= 0: all), ``top_p`` (>= 1: all) and ``min_p`` (0: all) are numbers
     or, for settings of each row's own, vectors: int32 for ``top_k``, fp32 for the others.  They apply in this
