@@ -156,12 +156,6 @@ struct QueryRow {
   }
 };
 
-// What a lane needs to know of its unit of a tile.
-struct UnitInfo {
-  float ks, vs;
-  bool ok;   // the page is one of the cache's
-};
-
 // The table's entry for a unit below the key limit (-1 beyond), and whether it is a page of the cache; page 0 stands in.
 __device__ inline int32_t kv8_entry(const Kv8Args& a, const int32_t* row, int unit, int limit) {
   return unit * 16 < limit ? row[unit >> a.unit_shift] : -1;
