@@ -246,10 +246,10 @@ def launch(device: torch.device, what: str, fn, *args) -> None:
     current, and check its status.  The context manager that makes it current is entered only where it is not."""
     index = device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc, what)
 

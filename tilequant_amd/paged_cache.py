@@ -119,7 +119,7 @@ class BlockTables:
         nat.launch(dev, "tq_block_tables_step", nat.lib().tq_block_tables_step,
                    new_tokens.data_ptr(), nat.ptr(finished), *self._state, at, at + 4 * max_tokens, at + 8 * max_tokens,
                    granted.data_ptr(), rows, width, self.block_size, max_tokens)
-        return StepSlots(out[:max_tokens], out[max_tokens:2 * max_tokens], out[2 * max_tokens:], granted)
+        return StepSlots(*out.split((max_tokens, max_tokens, rows + 1)), granted)
 
 
 @lru_cache(maxsize=1024)
@@ -264,8 +264,12 @@ class PagedKVCache:
                 raise ValueError("max_length must not be negative")
             bound = min(bound, int(max_length))
         if out is None:
-            out = torch.empty((tokens, hq, dim), device=self.device, dtype=query.dtype) if query_start is None \
-                else torch.zeros((tokens, hq, dim), device=self.device, dtype=query.dtype)
+            if query_start is not None:
+                out = torch.zeros((tokens, hq, dim), device=self.device, dtype=query.dtype)
+            elif query.is_contiguous():
+                out = torch.empty_like(query)   # half a microsecond less than spelling it out
+            else:
+                out = torch.empty((tokens, hq, dim), device=self.device, dtype=query.dtype)
         else:
             self._rows("out", out, hq, query.dtype)
             if out.shape[0] != tokens:
