@@ -533,7 +533,8 @@ int tq_kv8_read(const tq_kv8_cache* cache, const int32_t* slots, int n, int dtyp
  *   out = softmax(scale * q k^T) v,  kv head h / (q_heads / kv_heads)
  * A query that sees no key gives zeros; keys whose table entry is not a page of
  * the cache are left out; q rows of no sequence, and queries past max_query of
- * their sequence, leave out as it was.  q, out: [tokens, q_heads, head_dim] with
+ * their sequence, leave out as it was, or with zero_rest != 0 (batch > 0) are
+ * written 0.  q, out: [tokens, q_heads, head_dim] with
  * strides per token / head, 16-byte aligned, strides multiples of 8; at most 128
  * query heads per kv head; batch * kv_heads <= 65535.  fp32 accumulation.  workspace =
  * tq_kv8_attention_workspace_elems() floats, 8-byte aligned (0: none needed). */
@@ -542,8 +543,8 @@ int64_t tq_kv8_attention_workspace_elems(int tokens, int batch, int q_heads, int
 int tq_kv8_attention(const tq_kv8_cache* cache, const void* q, int64_t q_stride_t, int64_t q_stride_h, int dtype,
                      const int32_t* table, int64_t table_stride, int width, const int32_t* lengths,
                      const int32_t* query_start, int tokens, int batch, int q_heads, int max_query, int max_len,
-                     float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* workspace,
-                     int64_t workspace_elems, void* stream);
+                     float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, int zero_rest,
+                     float* workspace, int64_t workspace_elems, void* stream);
 
 /* ---- warming the next decode GEMM's weights into the right L2 ---------------
  * On MI355X each of the 8 XCDs has its own L2, and workgroups are dealt to

@@ -369,6 +369,27 @@ def test_rows_and_lengths_outside_what_is_asked():
     assert (err[[0, 1, 3, 4]] <= tol[[0, 1, 3, 4]]).all() and bool((out[2] == 7).all())
 
 
+@pytest.mark.parametrize("lengths,news,before,behind", [([100, 64], [3, 2], 0, 3), ([100, 64], [3, 2], 2, 0), ([90, 80, 70], [60, 0, 50], 3, 200),
+                                                        ([5000], [4], 1, 70), ([5000], [150], 5, 9), ([0, 3], [0, 0], 0, 6)])
+def test_a_new_output_is_zero_where_no_query_is(lengths, news, before, behind):
+    """Rows before the first and behind the last sequence, and past max_query, in memory that held something else."""
+    c, table, q, starts, scale = attention_case(lengths, news, 6, 2, 128, 32, torch.bfloat16, seed=9)
+    filler = lambda n: torch.full((n, 6, 128), 2.0, dtype=q.dtype)   # noqa: E731
+    q = torch.cat([filler(before), q, filler(behind)])
+    starts = [s + before for s in starts]
+    longest = max(1, max(news))
+    for most in {longest, max(1, longest - 1)}:
+        torch.full((q.numel(),), float("nan"), dtype=q.dtype, device=DEV)    # what a new tensor may find
+        got = c.gpu.attend(1, q.to(DEV), i32(table), i32(lengths), scale=scale, query_start=i32(starts), max_query=most)
+        kept = torch.full((len(q), 6, 128), 7.0, dtype=q.dtype, device=DEV)
+        c.gpu.attend(1, q.to(DEV), i32(table), i32(lengths), scale=scale, query_start=i32(starts), max_query=most, out=kept)
+        none = torch.ones(len(q), dtype=torch.bool)
+        for a, n in zip(starts, news):
+            none[a:a + min(n, most)] = False
+        assert bool((kept[none.to(DEV)] == 7).all()) and not got[none.to(DEV)].any()
+        assert torch.equal(got[~none.to(DEV)], kept[~none.to(DEV)])
+
+
 def test_strided_queries_and_outputs():
     lengths = [130, 17]
     c, table, q, starts, scale = attention_case(lengths, [1, 1], 6, 2, 128, 16, torch.bfloat16, seed=12)

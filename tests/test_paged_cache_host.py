@@ -49,7 +49,7 @@ def test_append_and_read_refusals():
 def attention(cache_, *, q=FAKE, dtype=0, table=FAKE, ld=4, width=4, lengths=FAKE, starts=None, tokens=3, batch=3, heads=8,
               max_query=1, max_len=256, scale=0.1, out=FAKE, ws=None, ws_elems=0, st=1024, sh=128):
     return nat.load().tq_kv8_attention(cache_, q, st, sh, dtype, table, ld, width, lengths, starts, tokens, batch, heads,
-                                       max_query, max_len, scale, out, 1024, 128, ws, ws_elems, None)
+                                       max_query, max_len, scale, out, 1024, 128, 0, ws, ws_elems, None)
 
 
 def test_attention_refusals():

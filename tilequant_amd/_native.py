@@ -171,7 +171,7 @@ _SIGNATURES.update({
     "tq_kv8_read": (_i, [ctypes.POINTER(Kv8Cache), _p, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p]),
     "tq_kv8_attention_workspace_elems": (_i64, [_i, _i, _i, _i, _i, _i, _i]),
     "tq_kv8_attention": (_i, [ctypes.POINTER(Kv8Cache), _p, _i64, _i64, _i, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _i,
-                              ctypes.c_float, _p, _i64, _i64, _p, _i64, _p]),
+                              ctypes.c_float, _p, _i64, _i64, _i, _p, _i64, _p]),
     "tq_sample_tokens": (_i, [_p, _i64, _i, _i, _i, _p, _p, ctypes.c_float, _p, _i, _p, ctypes.c_float,
                               _p, ctypes.c_float, _p, _p, _i64, _p]),
     "tq_sample_workspace_elems": (_i64, [_i, _i]),

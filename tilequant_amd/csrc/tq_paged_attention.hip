@@ -48,6 +48,7 @@ struct Kv8Args {
   int pages, unit_shift, units;
   int len_cap;                  // the most tokens a sequence counts as having: the table's width, the caller's bound
   int n_splits, chunk;          // keys per split, a multiple of 64
+  int zero_rest;                // rows of no answered query are written 0
   int64_t head_bytes;           // bytes of one (page, head): units * 16 * D
   float scale_log2, scale_sign; // |scale| log2(e), its sign
 };
@@ -69,6 +70,25 @@ __device__ inline Kv8Seq kv8_seq(const Kv8Args& a, int b) {
   s.before = s.len - n;
   s.n = min(n, a.max_query);
   return s;
+}
+
+// The rows of one kv head that no answered query of sequence b takes (past max_query of it), and a share of those before
+// the first and behind the last sequence, written 0 by part `part` of `parts` of this sequence's workgroups.  (Filling
+// the whole output before took 7 of 138 us for 4 prompts of up to 2048 tokens, and a launch.)
+template <int D>
+__device__ inline void kv8_zero_rest(const Kv8Args& a, int b, int h, const Kv8Seq& sq, int part, int parts) {
+  const auto zero = [&](int64_t t0, int t1, int64_t step) {
+    for (int64_t t = t0; t < t1; t += step)
+      for (int i = threadIdx.x; i < a.G * (D / 8); i += blockDim.x)
+        *reinterpret_cast<u32x4*>(a.out + t * a.o_st + (int64_t)(h * a.G + i / (D / 8)) * a.o_sh + i % (D / 8) * 8) =
+            u32x4{0, 0, 0, 0};
+  };
+  const int first = min(max(a.query_start[0], 0), a.tokens), last = min(max(a.query_start[a.batch], 0), a.tokens);
+  const int next = min(max(a.query_start[b + 1], sq.first), a.tokens);
+  const int64_t share = (int64_t)b * parts + part, shares = (int64_t)a.batch * parts;
+  zero((int64_t)sq.first + sq.n + part, next, parts);
+  zero(share, first, shares);
+  zero(last + share, a.tokens, shares);
 }
 
 __device__ inline float g4_sum(float x) {   // over lanes l, l ^ 16, l ^ 32, l ^ 48; the same association in every lane
@@ -239,6 +259,7 @@ kv8_split_kernel(Kv8Args a) {
   const int b = blockIdx.y / a.kv_heads, h = blockIdx.y - b * a.kv_heads;
   const Kv8Seq sq = kv8_seq(a, b);
   const int rows = sq.n * a.G, r0 = blockIdx.z * kKv8Rows;
+  if (a.zero_rest && split == 0) kv8_zero_rest<D>(a, b, h, sq, blockIdx.z, gridDim.z);
   if (r0 >= rows) return;
   const int last_i = min(sq.n - 1, (r0 + kKv8Rows - 1) / a.G);
   const int hi = sq.before + last_i + 1;   // keys seen by the tile's last row (may be <= 0)
@@ -356,8 +377,9 @@ kv8_split_kernel(Kv8Args a) {
 // conflicts either way), two tiles deep, and every wave multiplies its rows with all of them.
 // The bound is instruction issue, two waves a SIMD: matrix instructions take 30% of the SIMDs' cycles, the vector
 // instructions (per tile and wave 170 of softmax, 32 of them exponentials, and 85 of widening) 52%.  4 prompts of 1500 to
-// 2048 tokens, 24 / 8 heads of 128: 137 us, 0.61 PFLOP/s of what the mask leaves; 512 tokens over 16384: 0.74; a large
-// fp16 product reaches 1.19.  48 rows a wave, or the next tile's scores beside this tile's softmax, spill (203 us and more).
+// 2048 tokens, 24 / 8 heads of 128: 131 us, 0.64 PFLOP/s of what the mask leaves; 512 tokens over 16384: 0.75; a large
+// fp16 product reaches 1.19.  48 rows a wave, or the next tile's scores beside this tile's softmax, spill (203 us and more);
+// 32 x 32 x 16 products, half as many, took 146.
 constexpr int kKv8Block = 128;   // rows per workgroup
 constexpr int kKv8Waves = 4;
 
@@ -376,6 +398,7 @@ kv8_block_kernel(Kv8Args a) {
   const int split = blockIdx.z;
   const Kv8Seq sq = kv8_seq(a, b);
   const int rows = sq.n * a.G;
+  if (a.zero_rest && split == 0) kv8_zero_rest<D>(a, b, h, sq, blockIdx.y, gridDim.y);
   // The last row tiles have the most keys: they go first, over all sequences and heads (4 prompts of up to 2048
   // tokens, 8 kv heads: 143 us when this was tried, 173 with all tiles of a head before the next head's).
   const int tiles = (rows + kKv8Block - 1) / kKv8Block;
@@ -703,7 +726,7 @@ extern "C" int tq_kv8_attention(const tq_kv8_cache* cache, const void* q, int64_
                                 int dtype, const int32_t* table, int64_t table_stride, int width,
                                 const int32_t* lengths, const int32_t* query_start, int tokens, int batch,
                                 int q_heads, int max_query, int max_len, float scale, void* out,
-                                int64_t out_stride_t, int64_t out_stride_h, float* workspace,
+                                int64_t out_stride_t, int64_t out_stride_h, int zero_rest, float* workspace,
                                 int64_t workspace_elems, void* stream) {
   if (dtype != TQ_DTYPE_BF16 && dtype != TQ_DTYPE_FP16) return TQ_ERR_DTYPE;
   if (cache == nullptr || cache->pages <= 0 || cache->kv_heads <= 0) return TQ_ERR_ARG;
@@ -739,7 +762,7 @@ extern "C" int tq_kv8_attention(const tq_kv8_cache* cache, const void* q, int64_
   a.max_query = max_query;
   a.pages = cache->pages; a.len_cap = (int)(max_len < room ? max_len : room); a.units = cache->block / 16;
   a.unit_shift = 31 - __builtin_clz((unsigned)a.units);
-  a.n_splits = p.n_splits; a.chunk = p.chunk;
+  a.n_splits = p.n_splits; a.chunk = p.chunk; a.zero_rest = zero_rest && query_start != nullptr;
   a.head_bytes = (int64_t)cache->block * cache->head_dim;
   a.scale_log2 = (scale < 0 ? -scale : scale) * kLog2e8;
   a.scale_sign = scale < 0 ? -1.0f : 1.0f;

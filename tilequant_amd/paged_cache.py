@@ -263,8 +263,9 @@ class PagedKVCache:
             if max_length < 0:
                 raise ValueError("max_length must not be negative")
             bound = min(bound, int(max_length))
+        zero_rest = out is None and query_start is not None
         if out is None:
-            if query_start is not None:
+            if batch == 0:
                 out = torch.zeros((tokens, hq, dim), device=self.device, dtype=query.dtype)
             elif query.is_contiguous():
                 out = torch.empty_like(query)   # half a microsecond less than spelling it out
@@ -282,5 +283,5 @@ class PagedKVCache:
                    self._layer(layer), query.data_ptr(), query.stride(0), query.stride(1), nat.dtype_code(query.dtype),
                    block_table.data_ptr(), max(block_table.stride(0), width), width, lengths.data_ptr(),
                    nat.ptr(query_start), tokens, batch, hq, max_query, bound, float(scale), out.data_ptr(), out.stride(0),
-                   out.stride(1), nat.ptr(workspace), workspace.numel() if workspace is not None else 0)
+                   out.stride(1), zero_rest, nat.ptr(workspace), workspace.numel() if workspace is not None else 0)
         return out
