@@ -27,7 +27,7 @@
 // in LDS.  Masses being integers, C does not change the answer.
 // Bounds, and what the four take at a vocabulary of 128256 (us): 256 fp32 rows of mixed settings 32 + 37 + 29 + 25, the
 // passes bound by memory (131 MB each at most, 4.1 TB/s in the first), the last by its slowest row's chain of steps; 64
-// bf16 rows, top-p alone 6 + 18 + 22 + 24, the weights in fp64 and again the steps; one row with top-k 3 + 8 + 2 + 5.  One
+// bf16 rows, top-p alone 6 + 18 + 21 + 24, the weights in fp64 and again the steps; one row with top-k 3 + 8 + 2 + 5.  One
 // workgroup per row throughout took 254 / 202 / 21.
 #include "tq_common.h"
 
@@ -77,6 +77,7 @@ struct SampleArgs {
   uint32_t* above;
   uint32_t* bin_count;  // [chunks][kSampBins]
   uint32_t* n_list;     // [1]
+  float* top;           // [1]: the row's maximum, where it is not greedy
   uint64_t* row_mass;   // [kSampBins + 2]: the row's bins, above_mass and above
   uint32_t* row_count;  // [kSampBins]
 };
@@ -760,7 +761,7 @@ struct Needed {
       return;
     }
     if (set.p < 1.0) {
-      const int b = bin_of_search(Search::from(set.p * (double)lo), bins, 0, 0);
+      const int b = lo == hi ? end : bin_of_search(Search::from(set.p * (double)lo), bins, 0, 0);
       range(1, b, end);
       const uint64_t through = bins.mass_before[end] + bins.mass[end];
       lo = bins.mass_before[b] < lo ? bins.mass_before[b] : lo;
@@ -1039,6 +1040,7 @@ sample_chunk_kernel(SampleArgs a) {
   if (set.greedy()) return;
   RowMaxima<kChunkThreads> maxima;
   const float top = maxima.load(a, b, sh);
+  if (c == 0 && t == 0) a.top[b] = top;
   if (top == -INFINITY) return;
   const SampleRow r(top, set.T);
   int v0, v1;
@@ -1134,8 +1136,7 @@ sample_gather_kernel(SampleArgs a) {
   const SampleSettings set(a, b);
   if (set.greedy() || set.by_list()) return;
   const typename IN::T* row = static_cast<const typename IN::T*>(a.x) + (int64_t)b * a.ld;
-  RowMaxima<kChunkThreads> maxima;
-  const float top = maxima.load(a, b, sh);
+  const float top = a.top[b];
   if (top == -INFINITY) return;
   const SampleRow r(top, set.T);
   uint64_t above, above_mass;
@@ -1170,8 +1171,7 @@ sample_finish_kernel(SampleArgs a) {
     if (t == 0) a.out[b] = best.i;
     return;
   }
-  RowMaxima<kSampThreads> maxima;
-  const float top = maxima.load(a, b, sh);
+  const float top = a.top[b];
   int token;
   if (top == -INFINITY) {
     token = argmax_row<IN, kSampThreads>(row, a.vocab, 0, row_vectors<IN>(row, a.vocab), sh).i;
@@ -1248,6 +1248,7 @@ static int sample_launch(SampleArgs a, const SamplePlan& p, uint64_t* ws, hipStr
   a.above = a.row_count + (int64_t)a.rows * kSampBins;
   a.best = reinterpret_cast<int32_t*>(a.above + n);
   a.n_list = reinterpret_cast<uint32_t*>(a.best + n);
+  a.top = reinterpret_cast<float*>(a.n_list + a.rows);
   TQ_RETURN_IF_HIP_ERROR((allow_lds<sample_finish_kernel<IN>>(lds)));
   const dim3 grid(p.chunks, a.rows), block(kChunkThreads);
   hipLaunchKernelGGL(sample_max_kernel<IN>, grid, block, 0, s, a);
