@@ -129,8 +129,9 @@ def _attention_elems(*sizes: int) -> int:
 
 def paged_attention_workspace(tokens: int, batch: int, q_heads: int, kv_heads: int, head_dim: int, max_query: int,
                               max_length: int, device) -> Optional[torch.Tensor]:
-    """fp32 scratch for the split partials of ``PagedKVCache.attend``; None when the call needs none."""
-    elems = _attention_elems(tokens, batch, q_heads, kv_heads, head_dim, max_query, max_length)
+    """fp32 scratch for the split partials of ``PagedKVCache.attend`` (``max_length``: the bound it is called with, at
+    most the table's width in tokens); None when the call needs none."""
+    elems = _attention_elems(tokens, batch, q_heads, kv_heads, head_dim, min(max_query, tokens), max_length)
     return torch.empty((elems,), device=device, dtype=torch.float32) if elems else None
 
 
